@@ -72,8 +72,13 @@ typedef enum mhc_op {
   MHC_OP_DYNAMIC_WEIGHTS_FWD = 3,
   MHC_OP_DYNAMIC_WEIGHTS_BWD = 4,
   MHC_OP_HC_MIX_FWD = 5,
-  MHC_OP_HC_MIX_BWD = 6
+  MHC_OP_HC_MIX_BWD = 6,
+  MHC_OP_RMS_NORM_BWD = 7,    /* B is ignored, S is the number of rows */
+  MHC_OP_STREAM_NORM_BWD = 8
 } mhc_op;
+
+/* Type of the scales of an 8-bit output.  E8M0: a power of two as its biased exponent in one byte. */
+typedef enum mhc_scale_type { MHC_SCALE_F32 = 0, MHC_SCALE_E8M0 = 1 } mhc_scale_type;
 
 typedef void* mhc_stream_t; /* a cudaStream_t */
 typedef void* mhc_event_t;  /* a cudaEvent_t */
@@ -202,6 +207,76 @@ int mhc_add_residual_bwd_noalloc(const void* dH_new, const void* branch_output, 
                                  int64_t D, int dtype, mhc_stream_t stream);
 int64_t mhc_add_residual_bwd_noalloc_max_bytes(void);
 
+/* ---- Dropout with counter-based masks ---------------------------------------------
+ * y[r,d] = keep(r,d) * x[r,d] / (1 - p); a dropped element is 0 whatever x held.  keep is a function of
+ * (rng[0] = seed, rng[1] = offset, row_offset + r, d) alone, so no mask is stored: the backward is the
+ * same call on the upstream gradient.  `rng` points to two int64 in device memory, read by the kernel
+ * (a captured call therefore sees what they hold when the graph is replayed).  An element is dropped
+ * with probability drop_threshold / 65536 (1 .. 65535), which is the p of the formula.  Column d of a
+ * row takes the 16-bit piece d % 8 (low half of word 0 first) of Philox4x32-10 with key = seed and
+ * counter = (d / 8, row, offset low, offset high); row_offset + rows <= 2^32.
+ * The reference has no dropout; this replaces torch's on the branch output.  y may equal x. */
+int mhc_counter_dropout(const void* x, const int64_t* rng, int drop_threshold, int64_t row_offset, void* y,
+                        int64_t rows, int64_t D, int dtype, mhc_stream_t stream);
+
+/* Add residual with that dropout applied to branch_output on its way in (row = b * S + s):
+ * H_new = H + H_post * dropout(branch_output), with H the materialised residual mix (H_res NULL) or,
+ * where H_res is given, H_res @ H recomputed from the state as in mhc_add_residual_mix_fwd.
+ * pool_partials as in mhc_add_residual_pool_fwd, or NULL. */
+int mhc_add_residual_dropout_fwd(const void* H, const float* H_res, const void* branch_output,
+                                 const float* H_post, const int64_t* rng, int drop_threshold,
+                                 int64_t row_offset, void* H_new, float* pool_partials, int64_t B, int64_t S,
+                                 int64_t D, int dtype, mhc_stream_t stream);
+/* Its backward: d_branch_output goes through the same mask, dH_post sums over the dropped branch output.
+ * Scratch of MHC_OP_ADD_RESIDUAL_BWD, `tickets` as in mhc_add_residual_bwd. */
+int mhc_add_residual_dropout_bwd(const void* dH_new, const void* branch_output, const float* H_post,
+                                 const int64_t* rng, int drop_threshold, int64_t row_offset,
+                                 void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
+                                 int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype,
+                                 mhc_stream_t stream);
+
+/* ---- Root-mean-square norm -----------------------------------------------------------
+ * s = x (through the dropout above where drop_threshold != 0) + residual (may be NULL);
+ * rstd = 1 / sqrt(mean_d s^2 + eps);  y = s * rstd * weight.
+ * weight: [D] fp32 or of the activation type (weight_dtype), or NULL for ones.  sum_out (s rounded to
+ * the activation type; what the backward reads) and rstd [rows] fp32 may be NULL.  s is normalised
+ * as computed, before that rounding.  The reference leaves norms to the caller. */
+int mhc_add_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
+                         const int64_t* rng, int drop_threshold, int64_t row_offset, void* sum_out, void* y,
+                         float* rstd, int64_t rows, int64_t D, int dtype, float eps, mhc_stream_t stream);
+
+/* The same with y as e4m3 bytes q [rows, D] and one scale per row (group 0) or per `group` columns (32, 64
+ * or 128; the last group of a row may be shorter): scale = max(max|y| / 448, 2^-126), rounded up to a power
+ * of two for MHC_SCALE_E8M0; q = y / scale to nearest even.  scales: [rows, max(1, ceil(D / group))].
+ * A group that holds a NaN, or an infinity, has a scale of NaN (E8M0: code 255) or infinity. */
+int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
+                               void* sum_out, void* q, void* scales, int64_t group, int scale_type,
+                               int64_t rows, int64_t D, int dtype, float eps, mhc_stream_t stream);
+
+/* Gradients of mhc_add_rms_norm_fwd.  dsum: gradient of sum_out, or NULL.  s: sum_out (x itself where there
+ * was neither residual nor dropout).  dx is also the residual's gradient; with dropout dx is the
+ * gradient behind the mask and dresidual (may be NULL) the one before it.  dweight [D] of weight_dtype, or
+ * NULL: a fixed-order sum over the rows. */
+int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* s, const float* rstd, const void* weight,
+                     int weight_dtype, const int64_t* rng, int drop_threshold, int64_t row_offset, void* dx,
+                     void* dresidual, void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows,
+                     int64_t D, int dtype, mhc_stream_t stream);
+
+/* Norm of the mixed streams in the kernel that mixes them: b = sum_n H_pre[n] H[n]; y = norm(b) * weight.
+ * branch_input (b rounded to the activation type) and rstd [B, S] may be NULL.  Fuses the first half of
+ * stream_mix_forward (src/mhc/_kernels.py:617-652) with the norm its caller runs on branch_input. */
+int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
+                        void* branch_input, void* y, float* rstd, int64_t B, int64_t S, int64_t D, int dtype,
+                        float eps, mhc_stream_t stream);
+int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype, void* q,
+                              void* scales, int64_t group, int scale_type, int64_t B, int64_t S, int64_t D,
+                              int dtype, float eps, mhc_stream_t stream);
+/* dH [B,S,4,D], dH_pre [B,4] fp32 and dweight (may be NULL) from dy and H; the mix is recomputed. */
+int mhc_stream_norm_bwd(const void* dy, const void* H, const float* H_pre, const float* rstd,
+                        const void* weight, int weight_dtype, void* dH, float* dH_pre, void* dweight,
+                        void* scratch, int64_t scratch_bytes, int64_t B, int64_t S, int64_t D, int dtype,
+                        mhc_stream_t stream);
+
 /* ---- Sequence mean-pool ---------------------------------------------------------
  * x[b, n*D + d] = (1/S) sum_s H[b,s,n,d], fp32 output.
  * Replaces H.mean(dim=1).reshape(B, 4*D), src/mhc/module.py:123. */
@@ -262,6 +337,17 @@ int mhc_hc_mix_fwd(const void* H, const float* phi, const float* H_pre_base, con
                    const float* pooled_partials, int64_t pooled_chunks, void* scratch,
                    int64_t scratch_bytes, int32_t* tickets, int64_t B, int64_t S, int64_t D,
                    int dtype, int iters, float eps, mhc_stream_t stream);
+
+/* The same with the norm of branch_input fused into its last kernel: y = norm(branch_input) * norm_weight and
+ * rstd [B, S] are written beside branch_input, which mhc_rms_norm_bwd needs (it turns the gradient of y
+ * into the d_branch_input of mhc_hc_mix_bwd).  H_residual is never written. */
+int mhc_hc_mix_norm_fwd(const void* H, const float* phi, const float* H_pre_base, const float* H_post_base,
+                        const float* H_res_base, const float* alpha_pre, const float* alpha_post,
+                        const float* alpha_res, const void* norm_weight, int norm_weight_dtype, float norm_eps,
+                        float* x, float* H_pre, float* H_post, float* H_res, float* saved, void* branch_input,
+                        void* y, float* rstd, const float* pooled_partials, int64_t pooled_chunks,
+                        void* scratch, int64_t scratch_bytes, int32_t* tickets, int64_t B, int64_t S,
+                        int64_t D, int dtype, int iters, float eps, mhc_stream_t stream);
 
 /* Backward of the same chain in one call.  In: gradients of branch_input, H_residual and H_post
  * plus what the forward left (H, x, saved, H_pre, H_res).  Out: dH (including grad_x / S, i.e.

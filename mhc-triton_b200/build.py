@@ -15,8 +15,9 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "mhc", "libmhc_b200.so")
-SOURCES = ["api.cu", "sinkhorn.cu", "stream.cu", "weights.cu", "weights_rows.cu", "weights_rows_tc.cu", "fused.cu", "noalloc.cu"]
-HEADERS = ["common.cuh", "launch.h", os.path.join("..", "..", "include", "mhc_b200.h")]
+SOURCES = ["api.cu", "sinkhorn.cu", "stream.cu", "weights.cu", "weights_rows.cu", "weights_rows_tc.cu", "fused.cu", "noalloc.cu",
+           "norm.cu", "dropout.cu"]
+HEADERS = ["common.cuh", "launch.h", "rng.cuh", os.path.join("..", "..", "include", "mhc_b200.h")]
 
 
 def nvcc_path():

@@ -11,12 +11,15 @@
 
 using namespace mhc;
 
-extern "C" int mhc_hc_mix_fwd(const void* H, const float* phi, const float* H_pre_base, const float* H_post_base,
+// What the forward of the norm variant adds: the norm of branch_input in the kernel that forms it.
+struct NormTail { const void* weight; int wdtype; float eps; void* y; float* rstd; };
+
+static int hc_mix_fwd_impl(const void* H, const float* phi, const float* H_pre_base, const float* H_post_base,
                               const float* H_res_base, const float* alpha_pre, const float* alpha_post,
                               const float* alpha_res, float* x, float* H_pre, float* H_post, float* H_res,
                               float* saved, void* branch_input, void* H_residual, const float* pooled_partials,
                               int64_t pooled_chunks, void* scratch, int64_t scratch_bytes, int32_t* tickets,
-                              int64_t B, int64_t S, int64_t D, int dtype, int iters, float eps,
+                              int64_t B, int64_t S, int64_t D, int dtype, int iters, float eps, const NormTail* norm,
                               mhc_stream_t stream) {
   if (int e = check_bsd_pub("hc_mix_fwd", B, S, D, dtype)) return e;
   if (iters < 0) return fail(MHC_ERR_BAD_ARGUMENT, "hc_mix_fwd: iters < 0");
@@ -47,7 +50,44 @@ extern "C" int mhc_hc_mix_fwd(const void* H, const float* phi, const float* H_pr
                                alpha_pre, alpha_post, alpha_res, H_pre, H_post, H_res, saved, proj_part, B, 4 * D,
                                iters, eps, (int*)tickets, st))
     return e;
+  if (norm)
+    return stream_norm_fwd_impl(H, H_pre, norm->weight, norm->wdtype, branch_input, norm->y, norm->rstd, B, S, D, dtype,
+                                norm->eps, st);
   return stream_mix_fwd_impl(H, H_pre, H_res, branch_input, H_residual, B, S, D, dtype, st);
+}
+
+extern "C" int mhc_hc_mix_fwd(const void* H, const float* phi, const float* H_pre_base, const float* H_post_base,
+                              const float* H_res_base, const float* alpha_pre, const float* alpha_post,
+                              const float* alpha_res, float* x, float* H_pre, float* H_post, float* H_res,
+                              float* saved, void* branch_input, void* H_residual, const float* pooled_partials,
+                              int64_t pooled_chunks, void* scratch, int64_t scratch_bytes, int32_t* tickets,
+                              int64_t B, int64_t S, int64_t D, int dtype, int iters, float eps,
+                              mhc_stream_t stream) {
+  return hc_mix_fwd_impl(H, phi, H_pre_base, H_post_base, H_res_base, alpha_pre, alpha_post, alpha_res, x, H_pre, H_post,
+                         H_res, saved, branch_input, H_residual, pooled_partials, pooled_chunks, scratch, scratch_bytes,
+                         tickets, B, S, D, dtype, iters, eps, nullptr, stream);
+}
+
+extern "C" int mhc_hc_mix_norm_fwd(const void* H, const float* phi, const float* H_pre_base, const float* H_post_base,
+                                   const float* H_res_base, const float* alpha_pre, const float* alpha_post,
+                                   const float* alpha_res, const void* norm_weight, int norm_weight_dtype, float norm_eps,
+                                   float* x, float* H_pre, float* H_post, float* H_res, float* saved,
+                                   void* branch_input, void* y, float* rstd, const float* pooled_partials,
+                                   int64_t pooled_chunks, void* scratch, int64_t scratch_bytes, int32_t* tickets,
+                                   int64_t B, int64_t S, int64_t D, int dtype, int iters, float eps,
+                                   mhc_stream_t stream) {
+  const char* what = "hc_mix_norm_fwd";
+  if (int e = check_bsd_pub(what, B, S, D, dtype)) return e;
+  if (norm_weight && norm_weight_dtype != MHC_F32 && norm_weight_dtype != dtype)
+    return fail(MHC_ERR_BAD_DTYPE, "%s: the weight must be fp32 or of the activation type", what);
+  if (!(norm_eps >= 0.f)) return fail(MHC_ERR_BAD_ARGUMENT, "%s: norm_eps must not be negative", what);
+  if (rows_of(B, S) > kMaxGridItems) return fail(MHC_ERR_BAD_SHAPE, "%s: too many tokens", what);
+  if (B == 0) return MHC_OK;
+  if (!y || !rstd) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  const NormTail norm{norm_weight, norm_weight_dtype, norm_eps, y, rstd};
+  return hc_mix_fwd_impl(H, phi, H_pre_base, H_post_base, H_res_base, alpha_pre, alpha_post, alpha_res, x, H_pre, H_post,
+                         H_res, saved, branch_input, nullptr, pooled_partials, pooled_chunks, scratch, scratch_bytes,
+                         tickets, B, S, D, dtype, iters, eps, &norm, stream);
 }
 
 extern "C" int mhc_hc_mix_bwd(const void* d_branch_input, const void* dH_residual, const float* dH_post,

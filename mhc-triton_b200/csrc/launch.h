@@ -9,6 +9,7 @@
 
 #include "../../include/mhc_b200.h"
 #include "common.cuh"
+#include "rng.cuh"
 
 namespace mhc {
 
@@ -36,6 +37,21 @@ inline int64_t geo_slots(const Geo& g) { return (int64_t)g.nchunk * g.CG; }  // 
 
 // Pack width usable for a row length D of `dtype` given the pointers involved.
 int pick_vec(int dtype, int64_t D, std::initializer_list<const void*> ptrs);
+
+// Runs CALL with T and V naming the element type and the pack width.
+#define MHC_DISPATCH(dtype, vec, CALL)                                                      \
+  do {                                                                                      \
+    if ((dtype) == MHC_F32) {                                                               \
+      if ((vec) == 1) { using T = float; constexpr int V = 1; CALL; }                       \
+      else { using T = float; constexpr int V = 4; CALL; }                                  \
+    } else if ((dtype) == MHC_BF16) {                                                       \
+      if ((vec) == 1) { using T = __nv_bfloat16; constexpr int V = 1; CALL; }               \
+      else { using T = __nv_bfloat16; constexpr int V = 8; CALL; }                          \
+    } else {                                                                                \
+      if ((vec) == 1) { using T = __half; constexpr int V = 1; CALL; }                      \
+      else { using T = __half; constexpr int V = 8; CALL; }                                 \
+    }                                                                                       \
+  } while (0)
 
 // Programmatic dependent launch (on unless MHC_PDL=0 is set in the environment): every kernel of
 // this library may be scheduled while the previous kernel on the stream is still draining; each
@@ -116,6 +132,17 @@ int rows_fwd_tc_launch(const float* x, const float* phi, BiasPtrs bias, const fl
 int64_t rows_tc_bwd_scratch_floats(int64_t K);
 int rows_bwd_tc_launch(const float* x, const float* phi, const float* buf, float* phi_part, float* grad_x,
                        float* scratch, int64_t batch, int64_t K, int max_groups, cudaStream_t st, int* groups_used);
+
+// Norm and dropout (norm.cu, dropout.cu).
+inline int64_t rows_of(int64_t B, int64_t S) {  // B * S, or a count no check accepts where that overflows
+  return S > 0 && B > (1LL << 40) / S ? 1LL << 62 : B * S;
+}
+int make_drop(const char* what, const int64_t* rng, int threshold, int64_t row_offset, int64_t rows, Drop* out);
+int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D);
+int64_t stream_norm_bwd_scratch_bytes(int64_t B, int64_t S, int64_t D);
+int reduce_partials_impl(const float* part, int64_t B, int64_t slots, int W, float* out, cudaStream_t st, const char* what);
+int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, int wdtype, void* bi, void* y,
+                         float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st);
 
 int64_t weights_fwd_scratch_bytes(int64_t batch, int64_t K);
 int64_t weights_bwd_scratch_bytes(int64_t batch, int64_t K);

@@ -1,0 +1,495 @@
+// Root-mean-square norm of the rows a sub-layer reads, with what surrounds it fused in:
+//   s    = x (+ residual), x optionally through the counter-based dropout of rng.cuh     (Src::Add)
+//        = sum_n H_pre[n] H[n], the mix of the four streams                              (Src::Mix)
+//   rstd = 1 / sqrt(mean(s^2) + eps),  y = s * rstd * weight
+// y leaves in the activation type, or as e4m3 with one scale per row or per group of 32 / 64 / 128 columns.
+// Backward: with c = sum_d dy w s,  ds = rstd (dy w - s rstd^2 c / D) (+ the gradient that reached s directly),
+// dweight = sum_rows dy s rstd; dropout's mask is recomputed.  All sums, the norm and the scales are fp32; s is
+// normalised as computed, before it is rounded to the activation type for sum_out.
+#include "common.cuh"
+#include "launch.h"
+#include "rng.cuh"
+
+namespace mhc {
+
+enum class Src { Add, Mix };
+enum class Out { Plain, RowScale, GroupScale };
+
+constexpr float kE4m3Max = 448.f;
+constexpr float kMinScale = 1.17549435082228751e-38f;  // 2^-126: keeps 1 / scale finite for rows of zeros
+
+struct NormFwd {
+  const void* x;         // [rows, D], or H [rows, 4, D]
+  const void* res;       // [rows, D] or null
+  const float* hpre;     // [B, 4] (Mix)
+  const void* weight;    // [D] or null (ones)
+  int w_f32;             // weight is fp32 (else: the activation type)
+  void* sum_out;         // [rows, D] or null
+  void* y;               // [rows, D] activation type, or e4m3 bytes
+  void* scales;          // [rows, G] fp32 or e8m0 bytes
+  float* rstd;           // [rows] or null
+  int64_t rows, S, D;
+  int group;             // columns per scale (GroupScale)
+  int e8m0;
+  float eps;
+  Drop drop;
+};
+
+struct NormBwd {
+  const void* dy;        // [rows, D]
+  const void* dsum;      // [rows, D] or null: gradient that reaches s beside the norm
+  const void* s;         // [rows, D], or H [rows, 4, D]
+  const float* hpre;
+  const float* rstd;     // [rows]
+  const void* weight;
+  int w_f32;
+  void* dx;              // [rows, D], or dH [rows, 4, D]
+  void* dres;            // [rows, D] or null (dropout: the gradient before the mask)
+  float* dw_part;        // [ctas, D] or null
+  float* dpre_part;      // [B, chunks, 4] (Mix)
+  int64_t items, S, D;   // items: rows (Add), batch elements x chunks (Mix)
+  int64_t chunks;        // per batch element (Mix)
+  int tpc;               // tokens per chunk (Mix)
+  Drop drop;
+};
+
+template <typename T> __device__ __forceinline__ float load_w(const void* w, int w_f32, int64_t d) {
+  if (!w) return 1.f;
+  return w_f32 ? __ldg((const float*)w + d) : to_f32(__ldg((const T*)w + d));
+}
+
+// max that keeps NaN (fmaxf drops it): a row that holds one must not get a finite scale.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Scale of values whose largest magnitude is `amax`, and its reciprocal.  e8m0: the next power of two that is not
+// below amax / 448 (so nothing saturates), as its biased exponent; NaN and infinity become the NaN code 255.
+struct Scale { float inv; float f32; uint8_t code; };
+__device__ __forceinline__ Scale make_scale(float amax, int e8m0) {
+  float s = __fdiv_rn(amax, kE4m3Max);
+  s = s < kMinScale ? kMinScale : s;  // false for NaN
+  Scale r;
+  if (!e8m0) {
+    r.f32 = s;
+    r.inv = __fdiv_rn(1.f, s);
+    r.code = 0;
+    return r;
+  }
+  const uint32_t b = __float_as_uint(s);
+  uint32_t e = (b >> 23) + ((b & 0x7fffffu) ? 1u : 0u);
+  if (!(s < __int_as_float(0x7f800000))) e = 255;
+  r.code = (uint8_t)e;
+  r.f32 = e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float(e << 23);
+  r.inv = e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((254u - e) << 23);
+  return r;
+}
+__device__ __forceinline__ void store_scale(void* scales, int64_t i, const Scale& s, int e8m0) {
+  if (e8m0) ((uint8_t*)scales)[i] = s.code;
+  else ((float*)scales)[i] = s.f32;
+}
+
+// Sum (and NaN-keeping maximum) over a CTA; the result reaches every thread.  Fixed order.
+template <bool MAX>
+__device__ __forceinline__ void block_sum_max(float& sum, float& mx, float* sm) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    sm[warp] = sum;
+    if (MAX) sm[32 + warp] = mx;
+  }
+  __syncthreads();
+  float t = 0.f, m = 0.f;
+  for (int w = 0; w < nw; ++w) {
+    t += sm[w];
+    if (MAX) m = max_nan(m, sm[32 + w]);
+  }
+  sum = t;
+  mx = m;
+}
+
+// ------------------------------------------------------------------------------------- any width, any alignment
+// s[row, d], read element by element.
+template <typename T, Src SRC, bool DROP>
+__device__ __forceinline__ float src_at(const NormFwd& a, const DropKey& key, const float (&pre)[4], int64_t row, int64_t d) {
+  if constexpr (SRC == Src::Mix) {
+    const T* h = (const T*)a.x + row * 4 * a.D + d;
+    return ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + a.D))) + pre[2] * to_f32(__ldg(h + 2 * a.D))) +
+           pre[3] * to_f32(__ldg(h + 3 * a.D));
+  } else {
+    float v[1] = {to_f32(__ldg((const T*)a.x + row * a.D + d))};
+    if constexpr (DROP) drop_apply<1>(a.drop, drop_bits<1>(a.drop, key, row, d), v);
+    if (a.res) v[0] += to_f32(__ldg((const T*)a.res + row * a.D + d));
+    return v[0];
+  }
+}
+
+// One CTA of 256 threads per row; the row is read again for every pass over it.
+template <typename T, Src SRC, bool DROP, Out OUT>
+__global__ void __launch_bounds__(256)
+k_norm_any_fwd(NormFwd a) {
+  pdl_prologue();
+  __shared__ float sm[64];
+  const int64_t row = blockIdx.x, D = a.D;
+  float pre[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (SRC == Src::Mix) {
+#pragma unroll
+    for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + row / a.S * 4 + n);
+  }
+  DropKey key{};
+  if constexpr (DROP) key = drop_key(a.drop);
+  float ss = 0.f, mx = 0.f;
+  for (int64_t d = threadIdx.x; d < D; d += 256) {
+    const float v = src_at<T, SRC, DROP>(a, key, pre, row, d);
+    if (a.sum_out) ((T*)a.sum_out)[row * D + d] = from_f32<T>(v);
+    ss = fmaf(v, v, ss);
+    if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v * load_w<T>(a.weight, a.w_f32, d)));
+  }
+  block_sum_max<OUT == Out::RowScale>(ss, mx, sm);
+  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + a.eps));
+  if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
+  if constexpr (OUT == Out::Plain) {
+    for (int64_t d = threadIdx.x; d < D; d += 256)
+      ((T*)a.y)[row * D + d] =
+          from_f32<T>(src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d));
+  } else if constexpr (OUT == Out::RowScale) {
+    const Scale s = make_scale(mx * rstd, a.e8m0);
+    if (threadIdx.x == 0) store_scale(a.scales, row, s, a.e8m0);
+    for (int64_t d = threadIdx.x; d < D; d += 256) {
+      const float y = src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
+      ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y * s.inv, 0.f);
+    }
+  } else {  // a warp per group
+    const int64_t G = (D + a.group - 1) / a.group;
+    const int lane = threadIdx.x & 31;
+    for (int64_t g = threadIdx.x >> 5; g < G; g += 8) {
+      float y[4], m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t d = g * a.group + j * 32 + lane;
+        y[j] = 0.f;
+        if (j * 32 < a.group && d < D)
+          y[j] = src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
+        m = max_nan(m, fabsf(y[j]));
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const Scale s = make_scale(m, a.e8m0);
+      if (lane == 0) store_scale(a.scales, row * G + g, s, a.e8m0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t d = g * a.group + j * 32 + lane;
+        if (j * 32 < a.group && d < D) ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y[j] * s.inv, 0.f);
+      }
+    }
+  }
+}
+
+// Persistent CTAs of 256 threads: CTA i takes items i, i + grid, ...  An item is a row (Add), or a chunk of tokens of
+// one batch element (Mix), whose dH_pre it sums.  dweight's partial sums live in the CTA's own row of dw_part.
+template <typename T, Src SRC, bool DROP>
+__global__ void __launch_bounds__(256)
+k_norm_any_bwd(NormBwd a) {
+  pdl_prologue();
+  __shared__ float sm[64];
+  __shared__ float red[8 * 4];
+  const int64_t D = a.D;
+  DropKey key{};
+  if constexpr (DROP) key = drop_key(a.drop);
+  float* dw = a.dw_part ? a.dw_part + (int64_t)blockIdx.x * D : nullptr;
+  if (dw)
+    for (int64_t d = threadIdx.x; d < D; d += 256) dw[d] = 0.f;
+  for (int64_t it = blockIdx.x; it < a.items; it += gridDim.x) {
+    int64_t r0 = it, r1 = it + 1;
+    float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (SRC == Src::Mix) {
+      const int64_t b = it / a.chunks, c = it % a.chunks;
+      r0 = b * a.S + c * a.tpc;
+      r1 = min(r0 + a.tpc, (b + 1) * a.S);
+#pragma unroll
+      for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + b * 4 + n);
+    }
+    for (int64_t row = r0; row < r1; ++row) {
+      const float rstd = __ldg(a.rstd + row);
+      auto s_at = [&](int64_t d) -> float {
+        if constexpr (SRC == Src::Mix) {
+          const T* h = (const T*)a.s + row * 4 * D + d;
+          return ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + D))) + pre[2] * to_f32(__ldg(h + 2 * D))) +
+                 pre[3] * to_f32(__ldg(h + 3 * D));
+        } else {
+          return to_f32(__ldg((const T*)a.s + row * D + d));
+        }
+      };
+      float c = 0.f, unused = 0.f;
+      for (int64_t d = threadIdx.x; d < D; d += 256) {
+        const float dy = to_f32(__ldg((const T*)a.dy + row * D + d)), s = s_at(d);
+        c = fmaf(dy * load_w<T>(a.weight, a.w_f32, d), s, c);
+        if (dw) dw[d] = fmaf(dy, s * rstd, dw[d]);
+      }
+      __syncthreads();  // the previous row's readers of sm are done
+      block_sum_max<false>(c, unused, sm);
+      const float k = c * rstd * rstd * rstd / (float)D;
+      for (int64_t d = threadIdx.x; d < D; d += 256) {
+        const float dy = to_f32(__ldg((const T*)a.dy + row * D + d));
+        float g[1] = {rstd * (dy * load_w<T>(a.weight, a.w_f32, d)) - s_at(d) * k};
+        if constexpr (SRC == Src::Mix) {
+          const T* h = (const T*)a.s + row * 4 * D + d;
+          T* o = (T*)a.dx + row * 4 * D + d;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            acc[n] = fmaf(g[0], to_f32(__ldg(h + n * D)), acc[n]);
+            o[n * D] = from_f32<T>(pre[n] * g[0]);
+          }
+        } else {
+          if (a.dsum) g[0] += to_f32(__ldg((const T*)a.dsum + row * D + d));
+          if constexpr (DROP) {
+            if (a.dres) ((T*)a.dres)[row * D + d] = from_f32<T>(g[0]);
+            drop_apply<1>(a.drop, drop_bits<1>(a.drop, key, row, d), g);
+          }
+          ((T*)a.dx)[row * D + d] = from_f32<T>(g[0]);
+        }
+      }
+    }
+    if constexpr (SRC == Src::Mix) {
+      __syncthreads();
+      block_reduce_store<4>(acc, a.dpre_part + it * 4, red);
+    }
+  }
+}
+
+// out[d] = sum_i part[i, d] in fp64, fixed order: eight threads per column take rows i, i + 8, ..., joined in order.
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_norm_dweight(const float* __restrict__ part, int64_t n, int64_t D, T* __restrict__ out) {
+  pdl_prologue();
+  __shared__ double sm[8][32];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t d = (int64_t)blockIdx.x * 32 + c;
+  double t = 0.0;
+  if (d < D)
+    for (int64_t i = g; i < n; i += 8) t += (double)__ldg(part + i * D + d);
+  sm[g][c] = t;
+  __syncthreads();
+  if (g == 0 && d < D) {
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += sm[j][c];
+    out[d] = from_f32<T>((float)s);
+  }
+}
+
+// --------------------------------------------------------------------------------------------------- host side
+// CTAs of the backward: enough to fill the device twice over; each leaves one row of dweight partial sums.
+static int64_t bwd_ctas(int64_t items) {
+  const int64_t most = 2 * (int64_t)sm_count();
+  return items < most ? items : most;
+}
+constexpr int kMixTpc = 8;  // tokens per chunk of the stream-norm backward
+static int64_t mix_chunks(int64_t S) { return (S + kMixTpc - 1) / kMixTpc; }
+
+int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D) { return bwd_ctas(rows) * D * (int64_t)sizeof(float); }
+int64_t stream_norm_bwd_scratch_bytes(int64_t B, int64_t S, int64_t D) {
+  return (bwd_ctas(B * mix_chunks(S)) * D + B * mix_chunks(S) * 4) * (int64_t)sizeof(float);
+}
+
+#define MHC_TYPE_DISPATCH(dtype, CALL)                             \
+  do {                                                             \
+    if ((dtype) == MHC_F32) { using T = float; CALL; }             \
+    else if ((dtype) == MHC_BF16) { using T = __nv_bfloat16; CALL; } \
+    else { using T = __half; CALL; }                               \
+  } while (0)
+
+// Arguments common to all entry points of this file.
+static int check_norm(const char* what, int64_t rows, int64_t D, int dtype, const void* weight, int wdtype) {
+  if (int e = check_bsd_pub(what, 1, 0, D, dtype)) return e;
+  if (rows < 0 || rows > kMaxGridItems) return fail(MHC_ERR_BAD_SHAPE, "%s: rows %lld out of range", what, (long long)rows);
+  if (weight && wdtype != MHC_F32 && wdtype != dtype)
+    return fail(MHC_ERR_BAD_DTYPE, "%s: the weight must be fp32 or of the activation type", what);
+  return MHC_OK;
+}
+
+static int check_quant(const char* what, int64_t group, int scale_type) {
+  if (group != 0 && group != 32 && group != 64 && group != 128)
+    return fail(MHC_ERR_BAD_ARGUMENT, "%s: group %lld is not 0 (row), 32, 64 or 128", what, (long long)group);
+  if (scale_type != MHC_SCALE_F32 && scale_type != MHC_SCALE_E8M0)
+    return fail(MHC_ERR_BAD_ARGUMENT, "%s: unknown scale type %d", what, scale_type);
+  return MHC_OK;
+}
+
+template <Src SRC, bool DROP, Out OUT>
+static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_t st) {
+  ProfScope ps(SRC == Src::Mix ? "k_stream_norm_fwd" : "k_rms_norm_fwd", st);
+  MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_fwd<T, SRC, DROP, OUT>, (unsigned)a.rows, 256, 0, st, a)));
+  return check_launch(what);
+}
+
+template <Src SRC, bool DROP>
+static int launch_bwd(const char* what, const NormBwd& a, int64_t ctas, int dtype, cudaStream_t st) {
+  ProfScope ps(SRC == Src::Mix ? "k_stream_norm_bwd" : "k_rms_norm_bwd", st);
+  MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_bwd<T, SRC, DROP>, (unsigned)ctas, 256, 0, st, a)));
+  return check_launch(what);
+}
+
+static int finish_dweight(const char* what, const float* part, int64_t ctas, int64_t D, void* dweight, int wdtype,
+                          cudaStream_t st) {
+  ProfScope ps("k_norm_dweight", st);
+  MHC_TYPE_DISPATCH(wdtype, (launch_k(k_norm_dweight<T>, (unsigned)((D + 31) / 32), 256, 0, st, part, ctas, D, (T*)dweight)));
+  return check_launch(what);
+}
+
+int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, int wdtype, void* bi, void* y,
+                         float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st) {
+  NormFwd a{};
+  a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = wdtype == MHC_F32; a.sum_out = bi; a.y = y; a.rstd = rstd;
+  a.rows = B * S; a.S = S; a.D = D; a.eps = eps;
+  return launch_fwd<Src::Mix, false, Out::Plain>("stream_norm_fwd", a, dtype, st);
+}
+
+}  // namespace mhc
+
+using namespace mhc;
+
+extern "C" int mhc_add_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
+                                    const int64_t* rng, int drop_threshold, int64_t row_offset, void* sum_out, void* y,
+                                    float* rstd, int64_t rows, int64_t D, int dtype, float eps, mhc_stream_t stream) {
+  const char* what = "add_rms_norm_fwd";
+  if (int e = check_norm(what, rows, D, dtype, weight, weight_dtype)) return e;
+  if (!(eps >= 0.f)) return fail(MHC_ERR_BAD_ARGUMENT, "%s: eps must not be negative", what);
+  NormFwd a{};
+  const bool drop = drop_threshold != 0;
+  if (drop)
+    if (int e = make_drop(what, rng, drop_threshold, row_offset, rows, &a.drop)) return e;
+  if (rows == 0 || D == 0) return MHC_OK;
+  if (!x || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = y;
+  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps;
+  cudaStream_t st = (cudaStream_t)stream;
+  return drop ? launch_fwd<Src::Add, true, Out::Plain>(what, a, dtype, st)
+              : launch_fwd<Src::Add, false, Out::Plain>(what, a, dtype, st);
+}
+
+extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
+                                          void* sum_out, void* q, void* scales, int64_t group, int scale_type,
+                                          int64_t rows, int64_t D, int dtype, float eps, mhc_stream_t stream) {
+  const char* what = "add_rms_norm_quant_fwd";
+  if (int e = check_norm(what, rows, D, dtype, weight, weight_dtype)) return e;
+  if (int e = check_quant(what, group, scale_type)) return e;
+  if (!(eps >= 0.f)) return fail(MHC_ERR_BAD_ARGUMENT, "%s: eps must not be negative", what);
+  if (rows == 0 || D == 0) return MHC_OK;
+  if (!x || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  NormFwd a{};
+  a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = q;
+  a.scales = scales; a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0;
+  a.rows = rows; a.S = 1; a.D = D; a.eps = eps;
+  cudaStream_t st = (cudaStream_t)stream;
+  return group ? launch_fwd<Src::Add, false, Out::GroupScale>(what, a, dtype, st)
+               : launch_fwd<Src::Add, false, Out::RowScale>(what, a, dtype, st);
+}
+
+extern "C" int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* s, const float* rstd, const void* weight,
+                                int weight_dtype, const int64_t* rng, int drop_threshold, int64_t row_offset, void* dx,
+                                void* dresidual, void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows,
+                                int64_t D, int dtype, mhc_stream_t stream) {
+  const char* what = "rms_norm_bwd";
+  if (int e = check_norm(what, rows, D, dtype, weight, weight_dtype)) return e;
+  NormBwd a{};
+  const bool drop = drop_threshold != 0;
+  if (drop)
+    if (int e = make_drop(what, rng, drop_threshold, row_offset, rows, &a.drop)) return e;
+  if (D == 0) return MHC_OK;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dweight && weight_dtype != MHC_F32 && weight_dtype != dtype)
+    return fail(MHC_ERR_BAD_DTYPE, "%s: the weight must be fp32 or of the activation type", what);
+  if (rows == 0) {
+    if (dweight && cudaMemsetAsync(dweight, 0, D * (weight_dtype == MHC_F32 ? 4 : 2), st) != cudaSuccess) return check_launch(what);
+    return MHC_OK;
+  }
+  if (dweight && scratch_bytes < rms_norm_bwd_scratch_bytes(rows, D))
+    return fail(MHC_ERR_SCRATCH_TOO_SMALL, "%s: scratch %lld < %lld bytes", what, (long long)scratch_bytes,
+                (long long)rms_norm_bwd_scratch_bytes(rows, D));
+  if (!dy || !s || !rstd || !dx || (dweight && !scratch)) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  if (!is_aligned_to(scratch, 4)) return fail(MHC_ERR_MISALIGNED, "%s: scratch must be 4-byte aligned", what);
+  if (!drop && dresidual) return fail(MHC_ERR_BAD_ARGUMENT, "%s: without dropout the residual's gradient is dx", what);
+  a.dy = dy; a.dsum = dsum; a.s = s; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dx;
+  a.dres = dresidual; a.dw_part = dweight ? (float*)scratch : nullptr; a.items = rows; a.S = 1; a.D = D;
+  const int64_t ctas = bwd_ctas(rows);
+  if (int e = drop ? launch_bwd<Src::Add, true>(what, a, ctas, dtype, st) : launch_bwd<Src::Add, false>(what, a, ctas, dtype, st))
+    return e;
+  return dweight ? finish_dweight(what, a.dw_part, ctas, D, dweight, weight_dtype, st) : MHC_OK;
+}
+
+extern "C" int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
+                                   void* branch_input, void* y, float* rstd, int64_t B, int64_t S, int64_t D, int dtype,
+                                   float eps, mhc_stream_t stream) {
+  const char* what = "stream_norm_fwd";
+  if (int e = check_bsd_pub(what, B, S, D, dtype)) return e;
+  if (int e = check_norm(what, rows_of(B, S), D, dtype, weight, weight_dtype)) return e;
+  if (!(eps >= 0.f)) return fail(MHC_ERR_BAD_ARGUMENT, "%s: eps must not be negative", what);
+  if (B == 0 || S == 0 || D == 0) return MHC_OK;
+  if (!H || !H_pre || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  return stream_norm_fwd_impl(H, H_pre, weight, weight_dtype, branch_input, y, rstd, B, S, D, dtype, eps,
+                              (cudaStream_t)stream);
+}
+
+extern "C" int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
+                                         void* q, void* scales, int64_t group, int scale_type, int64_t B, int64_t S,
+                                         int64_t D, int dtype, float eps, mhc_stream_t stream) {
+  const char* what = "stream_norm_quant_fwd";
+  if (int e = check_bsd_pub(what, B, S, D, dtype)) return e;
+  if (int e = check_norm(what, rows_of(B, S), D, dtype, weight, weight_dtype)) return e;
+  if (int e = check_quant(what, group, scale_type)) return e;
+  if (!(eps >= 0.f)) return fail(MHC_ERR_BAD_ARGUMENT, "%s: eps must not be negative", what);
+  if (B == 0 || S == 0 || D == 0) return MHC_OK;
+  if (!H || !H_pre || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  NormFwd a{};
+  a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q; a.scales = scales;
+  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps;
+  cudaStream_t st = (cudaStream_t)stream;
+  return group ? launch_fwd<Src::Mix, false, Out::GroupScale>(what, a, dtype, st)
+               : launch_fwd<Src::Mix, false, Out::RowScale>(what, a, dtype, st);
+}
+
+extern "C" int mhc_stream_norm_bwd(const void* dy, const void* H, const float* H_pre, const float* rstd,
+                                   const void* weight, int weight_dtype, void* dH, float* dH_pre, void* dweight,
+                                   void* scratch, int64_t scratch_bytes, int64_t B, int64_t S, int64_t D, int dtype,
+                                   mhc_stream_t stream) {
+  const char* what = "stream_norm_bwd";
+  if (int e = check_bsd_pub(what, B, S, D, dtype)) return e;
+  if (int e = check_norm(what, rows_of(B, S), D, dtype, weight, weight_dtype)) return e;
+  if (dweight && weight_dtype != MHC_F32 && weight_dtype != dtype)
+    return fail(MHC_ERR_BAD_DTYPE, "%s: the weight must be fp32 or of the activation type", what);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (B == 0 || S == 0 || D == 0) {
+    if (B > 0 && !dH_pre) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+    if ((B > 0 && cudaMemsetAsync(dH_pre, 0, B * 4 * sizeof(float), st) != cudaSuccess) ||
+        (dweight && D > 0 && cudaMemsetAsync(dweight, 0, D * (weight_dtype == MHC_F32 ? 4 : 2), st) != cudaSuccess))
+      return check_launch(what);
+    return MHC_OK;
+  }
+  if (scratch_bytes < stream_norm_bwd_scratch_bytes(B, S, D))
+    return fail(MHC_ERR_SCRATCH_TOO_SMALL, "%s: scratch %lld < %lld bytes", what, (long long)scratch_bytes,
+                (long long)stream_norm_bwd_scratch_bytes(B, S, D));
+  if (!dy || !H || !H_pre || !rstd || !dH || !dH_pre || !scratch) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  if (!is_aligned_to(scratch, 4)) return fail(MHC_ERR_MISALIGNED, "%s: scratch must be 4-byte aligned", what);
+  NormBwd a{};
+  a.dy = dy; a.s = H; a.hpre = H_pre; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dH;
+  a.chunks = mix_chunks(S); a.tpc = kMixTpc; a.items = B * a.chunks; a.S = S; a.D = D;
+  const int64_t ctas = bwd_ctas(a.items);
+  a.dpre_part = (float*)scratch;
+  a.dw_part = dweight ? a.dpre_part + a.items * 4 : nullptr;
+  if (int e = launch_bwd<Src::Mix, false>(what, a, ctas, dtype, st)) return e;
+  if (int e = reduce_partials_impl(a.dpre_part, B, a.chunks, 4, dH_pre, st, what)) return e;
+  return dweight ? finish_dweight(what, a.dw_part, ctas, D, dweight, weight_dtype, st) : MHC_OK;
+}

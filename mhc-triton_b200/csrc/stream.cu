@@ -7,6 +7,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "rng.cuh"
 
 namespace mhc {
 
@@ -178,13 +179,17 @@ k_stream_premix_fwd(const T* __restrict__ H, const float* __restrict__ Hpre, T* 
 }
 
 // ------------------------------------------------------------------------------ add residual
-template <typename T, int V>
+// DROP (here and in the other add-residual kernels): the branch output passes through the counter-based dropout of
+// rng.cuh on its way in (row = b * S + s); the mask is recomputed wherever it is needed.
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(MHC_MAX_COLS, MHC_ADDFWD_MINB)
 k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const float* __restrict__ Hpost,
-                   T* __restrict__ Hn, Geo g) {
+                   T* __restrict__ Hn, Geo g, Drop drop) {
   pdl_prologue();
   const Item it = decode_item(g);
   if (it.col >= g.DV) return;
+  DropKey key{};
+  if constexpr (DROP) key = drop_key(drop);
   float p[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -201,6 +206,7 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
       [&](const B5& u, int64_t s) {
         float y[V], x[V];
         unpack<T, V>(u.p[4], y);
+        if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
         T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -228,10 +234,10 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
 #ifndef MHC_ADDPOOL_STAGES
 #define MHC_ADDPOOL_STAGES 4
 #endif
-template <typename T, int V>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(MHC_MAX_COLS, 2)
 k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const float* __restrict__ Hpost,
-                        T* __restrict__ Hn, float* __restrict__ pool, Geo g) {
+                        T* __restrict__ Hn, float* __restrict__ pool, Geo g, Drop drop) {
   extern __shared__ __align__(16) float sm[];  // [2*V][sub][cols], used when several tokens are walked abreast
   pdl_prologue();
   const Item it = decode_item(g);
@@ -243,6 +249,8 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
     for (int e = 0; e < V; ++e) acc[n][e] = 0.f;
   const bool live = it.col < g.DV;
   if (live) {
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(drop);
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -256,6 +264,7 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
     auto compute = [&](const B5& u, int64_t s) {
       float y[V], x[V];
       unpack<T, V>(u.p[4], y);
+      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
       T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -331,10 +340,10 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
 #define MHC_ADDMIXPOOL_MINB 2
 #endif
 
-template <typename T, int V, bool POOL>
+template <typename T, int V, bool POOL, bool DROP>
 __global__ void __launch_bounds__(MHC_MAX_COLS, POOL ? MHC_ADDMIXPOOL_MINB : MHC_ADDMIX_MINB)
 k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, const T* __restrict__ bo,
-                       const float* __restrict__ Hpost, T* __restrict__ Hn, float* __restrict__ pool, Geo g) {
+                       const float* __restrict__ Hpost, T* __restrict__ Hn, float* __restrict__ pool, Geo g, Drop drop) {
   extern __shared__ __align__(16) float sm[];  // POOL: [2*V][sub][cols]
   pdl_prologue();
   const Item it = decode_item(g);
@@ -349,6 +358,8 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
   const bool live = it.col < g.DV;
   if (!POOL && !live) return;
   if (live) {
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(drop);
     float p[4], R[16];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -364,6 +375,7 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
     auto compute = [&](const B5& u, int64_t s) {
       float x[4][V], y[V], o[V];
       unpack<T, V>(u.p[4], y);
+      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
 #pragma unroll
       for (int n = 0; n < 4; ++n) unpack<T, V>(u.p[n], x[n]);
       T* op = Hn + (tok + s) * 4 * D + c0;
@@ -457,10 +469,11 @@ __device__ __forceinline__ void finish_partials(const float* __restrict__ part, 
 #ifndef MHC_ADDBWD_PIPE
 #define MHC_ADDBWD_PIPE 1
 #endif
-template <typename T, int V>
+template <typename T, int V, bool DROP>
 __global__ void __launch_bounds__(MHC_MAX_COLS, MHC_ADDBWD_MINB)
 k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const float* __restrict__ Hpost,
-                   T* __restrict__ dbo, float* __restrict__ part, Geo g, int* tickets, float* __restrict__ dH_post) {
+                   T* __restrict__ dbo, float* __restrict__ part, Geo g, int* tickets, float* __restrict__ dH_post,
+                   Drop drop) {
   pdl_prologue();
   __shared__ __align__(8) float red[32 * 20];
   const Item it = decode_item(g);
@@ -470,6 +483,8 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
     const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
+    DropKey key{};
+    if constexpr (DROP) key = drop_key(drop);
     using B5 = Bundle<T, V, 5>;
     for_tokens<MHC_ADDBWD_PIPE != 0, B5>(
         it.s0 + it.sub, it.s1, g.sub,
@@ -482,6 +497,11 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
         [&](const B5& u, int64_t s) {
           float y[V], z[V], x[V];
           unpack<T, V>(u.p[4], y);
+          DropBits<V> bits{};
+          if constexpr (DROP) {
+            bits = drop_bits<V>(drop, key, tok + s, c0);
+            drop_apply<V>(drop, bits, y);
+          }
 #pragma unroll
           for (int e = 0; e < V; ++e) z[e] = 0.f;
 #pragma unroll
@@ -493,6 +513,7 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
               acc[n] = fmaf(x[e], y[e], acc[n]);
             }
           }
+          if constexpr (DROP) drop_apply<V>(drop, bits, z);
           PackIO<T, V>::store(dbo + (tok + s) * D + c0, z);
         });
   }
@@ -824,20 +845,6 @@ static int check_grid(const char* what, int64_t items) {
   return MHC_OK;
 }
 
-#define MHC_DISPATCH(dtype, vec, CALL)                                                      \
-  do {                                                                                      \
-    if ((dtype) == MHC_F32) {                                                               \
-      if ((vec) == 1) { using T = float; constexpr int V = 1; CALL; }                       \
-      else { using T = float; constexpr int V = 4; CALL; }                                  \
-    } else if ((dtype) == MHC_BF16) {                                                       \
-      if ((vec) == 1) { using T = __nv_bfloat16; constexpr int V = 1; CALL; }               \
-      else { using T = __nv_bfloat16; constexpr int V = 8; CALL; }                          \
-    } else {                                                                                \
-      if ((vec) == 1) { using T = __half; constexpr int V = 1; CALL; }                      \
-      else { using T = __half; constexpr int V = 8; CALL; }                                 \
-    }                                                                                       \
-  } while (0)
-
 // Launch sequences shared by the single-op and the fused entry points.  Arguments are validated by
 // the callers; these pick the pack width, build the geometry and launch.
 int stream_mix_fwd_impl(const void* H, const float* H_pre, const float* H_res, void* bi, void* Hr, int64_t B, int64_t S,
@@ -943,6 +950,10 @@ static int launch_reduce(const float* part, int64_t B, int64_t slots, int W, int
   return check_launch(what);
 }
 
+int reduce_partials_impl(const float* part, int64_t B, int64_t slots, int W, float* out, cudaStream_t st, const char* what) {
+  return launch_reduce(part, B, slots, W, W, out, nullptr, st, what);
+}
+
 }  // namespace mhc
 
 using namespace mhc;
@@ -959,6 +970,8 @@ extern "C" int64_t mhc_scratch_bytes(int op, int64_t B, int64_t S, int64_t D, in
     case MHC_OP_DYNAMIC_WEIGHTS_FWD: return weights_fwd_scratch_bytes(B, 4 * D);
     case MHC_OP_DYNAMIC_WEIGHTS_BWD: return weights_bwd_scratch_bytes(B, 4 * D);
     case MHC_OP_HC_MIX_FWD: return meanpool_scratch_floats(B, S, D) * f + weights_fwd_scratch_bytes(B, 4 * D);
+    case MHC_OP_RMS_NORM_BWD: return rms_norm_bwd_scratch_bytes(S, D);
+    case MHC_OP_STREAM_NORM_BWD: return stream_norm_bwd_scratch_bytes(B, S, D);
     case MHC_OP_HC_MIX_BWD: return mix_bwd_scratch_floats(B, S, D) * f + weights_bwd_scratch_bytes(B, 4 * D);
   }
   return -1;
@@ -973,8 +986,16 @@ extern "C" int mhc_stream_mix_fwd(const void* H, const float* H_pre, const float
   return stream_mix_fwd_impl(H, H_pre, H_res, branch_input, H_residual, B, S, D, dtype, (cudaStream_t)stream);
 }
 
-extern "C" int mhc_add_residual_fwd(const void* H_residual, const void* branch_output, const float* H_post,
-                                    void* H_new, int64_t B, int64_t S, int64_t D, int dtype, mhc_stream_t stream) {
+// Launches kernel<T, V, DROP ...> with or without dropout; CALL names T, V and DROP.
+#define MHC_DROP_DISPATCH(dtype, vec, drop, CALL)                          \
+  do {                                                                     \
+    if (drop) { constexpr bool DROP = true; MHC_DISPATCH(dtype, vec, CALL); }   \
+    else { constexpr bool DROP = false; MHC_DISPATCH(dtype, vec, CALL); }       \
+  } while (0)
+
+static int add_residual_fwd_impl(const void* H_residual, const void* branch_output, const float* H_post,
+                                 const Drop* drop, void* H_new, int64_t B, int64_t S, int64_t D, int dtype,
+                                 mhc_stream_t stream) {
   if (int e = check_bsd("add_residual_fwd", B, S, D, dtype)) return e;
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H_residual || !branch_output || !H_post || !H_new) return fail(MHC_ERR_NULL_POINTER, "add_residual_fwd: null pointer");
@@ -986,10 +1007,16 @@ extern "C" int mhc_add_residual_fwd(const void* H_residual, const void* branch_o
   cudaStream_t st = (cudaStream_t)stream;
   {
     ProfScope ps("k_add_residual_fwd", st);
-    MHC_DISPATCH(dtype, vec, (launch_k(k_add_residual_fwd<T, V>, (unsigned)items, geo_block(g), 0, st, 
-                                 (const T*)H_residual, (const T*)branch_output, H_post, (T*)H_new, g)));
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_k(k_add_residual_fwd<T, V, DROP>, (unsigned)items, geo_block(g), 0, st,
+                                 (const T*)H_residual, (const T*)branch_output, H_post, (T*)H_new, g,
+                                 drop ? *drop : Drop{})));
   }
   return check_launch("add_residual_fwd");
+}
+
+extern "C" int mhc_add_residual_fwd(const void* H_residual, const void* branch_output, const float* H_post,
+                                    void* H_new, int64_t B, int64_t S, int64_t D, int dtype, mhc_stream_t stream) {
+  return add_residual_fwd_impl(H_residual, branch_output, H_post, nullptr, H_new, B, S, D, dtype, stream);
 }
 
 // Tokens per chunk of the add-residual kernels that also pool: MHC_TPC_ADDPOOL adjusted so that one batch
@@ -1008,9 +1035,9 @@ extern "C" int64_t mhc_add_residual_pool_chunks(int64_t S, int64_t D) {
   return (S + tpc - 1) / tpc;
 }
 
-extern "C" int mhc_add_residual_mix_fwd(const void* H, const float* H_res, const void* branch_output,
-                                        const float* H_post, void* H_new, float* pool_partials, int64_t B, int64_t S,
-                                        int64_t D, int dtype, mhc_stream_t stream) {
+static int add_residual_mix_fwd_impl(const void* H, const float* H_res, const void* branch_output,
+                                     const float* H_post, const Drop* drop, void* H_new, float* pool_partials,
+                                     int64_t B, int64_t S, int64_t D, int dtype, mhc_stream_t stream) {
   if (int e = check_bsd("add_residual_mix_fwd", B, S, D, dtype)) return e;
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H || !H_res || !branch_output || !H_post || !H_new)
@@ -1028,25 +1055,32 @@ extern "C" int mhc_add_residual_mix_fwd(const void* H, const float* H_res, const
     size_t smem = g.sub > 1 ? (size_t)2 * vec * geo_block(g) * sizeof(float) : 0;
     if (vec > 1 && MHC_ADDPOOL_STAGES > 0) smem = std::max(smem, (size_t)MHC_ADDPOOL_STAGES * 5 * 16 * geo_block(g));
     ProfScope ps("k_add_residual_mix_pool_fwd", st);
-    MHC_DISPATCH(dtype, vec, (launch_pool_k(k_add_residual_mix_fwd<T, V, true>, (unsigned)items, geo_block(g), smem, st,
-                                            (const T*)H, H_res, (const T*)branch_output, H_post, (T*)H_new, pool_partials, g)));
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_pool_k(k_add_residual_mix_fwd<T, V, true, DROP>, (unsigned)items,
+                                            geo_block(g), smem, st, (const T*)H, H_res, (const T*)branch_output, H_post,
+                                            (T*)H_new, pool_partials, g, drop ? *drop : Drop{})));
   } else {
     Geo g = make_geo(S, D, vec, GeoKind::Stream, MHC_TPC_ADDMIX);
     g.reverse = (MHC_REV_MASK >> 2) & 1;
     const int64_t items = B * geo_slots(g);
     if (int e = check_grid("add_residual_mix_fwd", items)) return e;
     ProfScope ps("k_add_residual_mix_fwd", st);
-    MHC_DISPATCH(dtype, vec, (launch_k(k_add_residual_mix_fwd<T, V, false>, (unsigned)items, geo_block(g), 0, st,
-                                       (const T*)H, H_res, (const T*)branch_output, H_post, (T*)H_new, (float*)nullptr,
-                                       g)));
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_k(k_add_residual_mix_fwd<T, V, false, DROP>, (unsigned)items,
+                                       geo_block(g), 0, st, (const T*)H, H_res, (const T*)branch_output, H_post,
+                                       (T*)H_new, (float*)nullptr, g, drop ? *drop : Drop{})));
   }
   return check_launch("add_residual_mix_fwd");
 }
 
+extern "C" int mhc_add_residual_mix_fwd(const void* H, const float* H_res, const void* branch_output,
+                                        const float* H_post, void* H_new, float* pool_partials, int64_t B, int64_t S,
+                                        int64_t D, int dtype, mhc_stream_t stream) {
+  return add_residual_mix_fwd_impl(H, H_res, branch_output, H_post, nullptr, H_new, pool_partials, B, S, D, dtype,
+                                   stream);
+}
 
-extern "C" int mhc_add_residual_pool_fwd(const void* H_residual, const void* branch_output, const float* H_post,
-                                         void* H_new, float* pool_partials, int64_t B, int64_t S, int64_t D, int dtype,
-                                         mhc_stream_t stream) {
+static int add_residual_pool_fwd_impl(const void* H_residual, const void* branch_output, const float* H_post,
+                                      const Drop* drop, void* H_new, float* pool_partials, int64_t B, int64_t S,
+                                      int64_t D, int dtype, mhc_stream_t stream) {
   if (int e = check_bsd("add_residual_pool_fwd", B, S, D, dtype)) return e;
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H_residual || !branch_output || !H_post || !H_new || !pool_partials)
@@ -1066,16 +1100,23 @@ extern "C" int mhc_add_residual_pool_fwd(const void* H_residual, const void* bra
   if (vec > 1 && MHC_ADDPOOL_STAGES > 0) smem = std::max(smem, (size_t)MHC_ADDPOOL_STAGES * 5 * 16 * geo_block(g));
   {
     ProfScope ps("k_add_residual_pool_fwd", st);
-    MHC_DISPATCH(dtype, vec, (launch_pool_k(k_add_residual_pool_fwd<T, V>, (unsigned)items, geo_block(g), smem, st,
-                                       (const T*)H_residual, (const T*)branch_output, H_post, (T*)H_new, pool_partials, g)));
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_pool_k(k_add_residual_pool_fwd<T, V, DROP>, (unsigned)items, geo_block(g),
+                                       smem, st, (const T*)H_residual, (const T*)branch_output, H_post, (T*)H_new,
+                                       pool_partials, g, drop ? *drop : Drop{})));
   }
   return check_launch("add_residual_pool_fwd");
 }
 
-extern "C" int mhc_add_residual_bwd(const void* dH_new, const void* branch_output, const float* H_post,
-                                    void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
-                                    int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype,
-                                    mhc_stream_t stream) {
+extern "C" int mhc_add_residual_pool_fwd(const void* H_residual, const void* branch_output, const float* H_post,
+                                         void* H_new, float* pool_partials, int64_t B, int64_t S, int64_t D, int dtype,
+                                         mhc_stream_t stream) {
+  return add_residual_pool_fwd_impl(H_residual, branch_output, H_post, nullptr, H_new, pool_partials, B, S, D, dtype,
+                                    stream);
+}
+
+static int add_residual_bwd_impl(const void* dH_new, const void* branch_output, const float* H_post, const Drop* drop,
+                                 void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
+                                 int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype, mhc_stream_t stream) {
   if (int e = check_bsd("add_residual_bwd", B, S, D, dtype)) return e;
   if (B == 0) return MHC_OK;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1100,13 +1141,48 @@ extern "C" int mhc_add_residual_bwd(const void* dH_new, const void* branch_outpu
   if (!ticket_finish_supported()) tickets = nullptr;
   {
     ProfScope ps("k_add_residual_bwd", st);
-    MHC_DISPATCH(dtype, vec, (launch_k(k_add_residual_bwd<T, V>, (unsigned)items, geo_block(g), 0, st, 
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_k(k_add_residual_bwd<T, V, DROP>, (unsigned)items, geo_block(g), 0, st,
                                  (const T*)dH_new, (const T*)branch_output, H_post, (T*)d_branch_output,
-                                 (float*)scratch, g, (int*)tickets, dH_post)));
+                                 (float*)scratch, g, (int*)tickets, dH_post, drop ? *drop : Drop{})));
   }
   if (int e = check_launch("add_residual_bwd")) return e;
   if (tickets) return MHC_OK;   // the last CTA of every batch element has written dH_post
   return launch_reduce((const float*)scratch, B, slots, 4, 4, dH_post, nullptr, st, "add_residual_bwd(reduce)");
+}
+
+extern "C" int mhc_add_residual_bwd(const void* dH_new, const void* branch_output, const float* H_post,
+                                    void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
+                                    int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype,
+                                    mhc_stream_t stream) {
+  return add_residual_bwd_impl(dH_new, branch_output, H_post, nullptr, d_branch_output, dH_post, scratch, scratch_bytes,
+                               tickets, B, S, D, dtype, stream);
+}
+
+extern "C" int mhc_add_residual_dropout_fwd(const void* H, const float* H_res, const void* branch_output,
+                                            const float* H_post, const int64_t* rng, int drop_threshold,
+                                            int64_t row_offset, void* H_new, float* pool_partials, int64_t B, int64_t S,
+                                            int64_t D, int dtype, mhc_stream_t stream) {
+  const char* what = "add_residual_dropout_fwd";
+  if (int e = check_bsd(what, B, S, D, dtype)) return e;
+  Drop drop;
+  if (int e = make_drop(what, rng, drop_threshold, row_offset, rows_of(B, S), &drop)) return e;
+  if (H_res) return add_residual_mix_fwd_impl(H, H_res, branch_output, H_post, &drop, H_new, pool_partials, B, S, D, dtype, stream);
+  if (pool_partials)
+    return add_residual_pool_fwd_impl(H, branch_output, H_post, &drop, H_new, pool_partials, B, S, D, dtype, stream);
+  return add_residual_fwd_impl(H, branch_output, H_post, &drop, H_new, B, S, D, dtype, stream);
+}
+
+extern "C" int mhc_add_residual_dropout_bwd(const void* dH_new, const void* branch_output, const float* H_post,
+                                            const int64_t* rng, int drop_threshold, int64_t row_offset,
+                                            void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
+                                            int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype,
+                                            mhc_stream_t stream) {
+  const char* what = "add_residual_dropout_bwd";
+  if (int e = check_bsd(what, B, S, D, dtype)) return e;
+  Drop drop;
+  if (int e = make_drop(what, rng, drop_threshold, row_offset, rows_of(B, S), &drop)) return e;
+  return add_residual_bwd_impl(dH_new, branch_output, H_post, &drop, d_branch_output, dH_post, scratch, scratch_bytes,
+                               tickets, B, S, D, dtype, stream);
 }
 
 static int mix_bwd_common(const char* what, int mode, const void* dbi, const void* dHr, const void* H,

@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from ._kernels import _check, _alpha_dev
+from ._kernels import _check, _alpha_dev, _norm_weight, _rows
 
 _ABS0 = {"zero": L.ABS0_ZERO, "plus_one": L.ABS0_PLUS_ONE}
 _abs_grad_at_zero = "zero"
@@ -187,3 +187,66 @@ def hc_mix_backward(d_branch_input, dH_residual, dH_post, H, x, phi, H_pre_base,
                (ready_event.cuda_event or None) if ready_event is not None else None, B, S, D, L.dtype_code(H),
                int(sinkhorn_iters), float(eps), _ABS0[_abs_grad_at_zero], 1 if accumulate else 0)
     return dH, g_phi, g_bias, g_alpha
+
+
+def add_residual_dropout_backward(dH_new, branch_output, H_post, rng, threshold: int, row_offset: int = 0):
+    """(dH_residual, d_branch_output, dH_post [B,4] fp32) of add_residual_dropout_forward; dH_residual IS dH_new."""
+    B, S, n, D = dH_new.shape
+    _check(n == 4 and tuple(branch_output.shape) == (B, S, D) and tuple(H_post.shape) == (B, 4), "shape mismatch")
+    L.require_same_device(dH_new, branch_output, H_post, rng)
+    dH_new = dH_new.contiguous()
+    branch_output = branch_output.to(dH_new.dtype).contiguous()
+    H_post = L.f32c(H_post)
+    d_bo = torch.empty_like(branch_output)
+    dH_post = torch.empty(B, 4, device=dH_new.device, dtype=torch.float32)
+    buf, nbytes = L.scratch(L.OP_ADD_RESIDUAL_BWD, B, S, D, dH_new)
+    L.call_on(dH_new, "mhc_add_residual_dropout_bwd", L.ptr(dH_new), L.ptr(branch_output), L.ptr(H_post), L.ptr(rng),
+              threshold, row_offset, L.ptr(d_bo), L.ptr(dH_post), L.ptr(buf), nbytes, L.tickets(dH_new, B), B, S, D,
+              L.dtype_code(dH_new))
+    return dH_new, d_bo, dH_post
+
+
+def rms_norm_backward(dy, dsum, s, rstd, weight=None, rng=None, threshold: int = 0, row_offset: int = 0,
+                      want_dresidual: bool = False, want_dweight: bool = True):
+    """(dx, dresidual, dweight) of add_rms_norm_forward from the gradients of y and of s (dsum, or None).  Without
+    dropout dresidual IS dx; dweight has the weight's type (None if not wanted)."""
+    D = s.shape[-1]
+    _check(dy.shape == s.shape and (dsum is None or dsum.shape == s.shape) and rstd.numel() == _rows(s), "shape mismatch")
+    L.require_same_device(s, dy, dsum, rstd, weight, rng)
+    s = s.contiguous()
+    dy = dy.to(s.dtype).contiguous()
+    dsum = None if dsum is None else dsum.to(s.dtype).contiguous()
+    w, wcode = _norm_weight(weight, s, D)
+    dx = torch.empty_like(s)
+    dres = torch.empty_like(s) if threshold and want_dresidual else None
+    dw, buf, nbytes = None, None, 0
+    if want_dweight and w is not None:
+        dw = torch.empty_like(w)
+        buf, nbytes = L.scratch(L.OP_RMS_NORM_BWD, 0, _rows(s), D, s)
+    L.call_on(s, "mhc_rms_norm_bwd", dy.data_ptr(), L.ptr(dsum), s.data_ptr(), rstd.data_ptr(), L.ptr(w), wcode,
+              L.ptr(rng), threshold, row_offset, dx.data_ptr(), L.ptr(dres), L.ptr(dw), L.ptr(buf), nbytes, _rows(s), D,
+              L.dtype_code(s))
+    if dw is not None and dw.dtype != weight.dtype:
+        dw = dw.to(weight.dtype)
+    return dx, (dres if threshold else dx), dw
+
+
+def stream_norm_backward(dy, H, H_pre, rstd, weight=None, want_dweight: bool = True):
+    """(dH, dH_pre [B,4] fp32, dweight or None) of stream_norm_forward."""
+    B, S, n, D = H.shape
+    _check(n == 4 and tuple(dy.shape) == (B, S, D) and tuple(H_pre.shape) == (B, 4) and rstd.numel() == B * S,
+           "shape mismatch")
+    L.require_same_device(H, dy, H_pre, rstd, weight)
+    H = H.contiguous()
+    dy = dy.to(H.dtype).contiguous()
+    H_pre = L.f32c(H_pre)
+    w, wcode = _norm_weight(weight, H, D)
+    dH = torch.empty_like(H)
+    dH_pre = torch.empty(B, 4, device=H.device, dtype=torch.float32)
+    dw = torch.empty_like(w) if want_dweight and w is not None else None
+    buf, nbytes = L.scratch(L.OP_STREAM_NORM_BWD, B, S, D, H)
+    L.call_on(H, "mhc_stream_norm_bwd", dy.data_ptr(), H.data_ptr(), H_pre.data_ptr(), rstd.data_ptr(), L.ptr(w), wcode,
+              dH.data_ptr(), dH_pre.data_ptr(), L.ptr(dw), L.ptr(buf), nbytes, B, S, D, L.dtype_code(H))
+    if dw is not None and dw.dtype != weight.dtype:
+        dw = dw.to(weight.dtype)
+    return dH, dH_pre, dw

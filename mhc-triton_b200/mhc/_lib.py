@@ -18,7 +18,8 @@ MHC_F32, MHC_BF16, MHC_F16 = 0, 1, 2
 _DTYPE_CODE = {torch.float32: MHC_F32, torch.bfloat16: MHC_BF16, torch.float16: MHC_F16}
 
 (OP_ADD_RESIDUAL_BWD, OP_STREAM_MIX_BWD, OP_MEANPOOL_FWD, OP_DYNAMIC_WEIGHTS_FWD, OP_DYNAMIC_WEIGHTS_BWD,
- OP_HC_MIX_FWD, OP_HC_MIX_BWD) = range(7)
+ OP_HC_MIX_FWD, OP_HC_MIX_BWD, OP_RMS_NORM_BWD, OP_STREAM_NORM_BWD) = range(9)
+SCALE_F32, SCALE_E8M0 = 0, 1
 
 ABS0_ZERO, ABS0_PLUS_ONE = 0, 1
 
@@ -41,6 +42,16 @@ _PROTOTYPES = {
     "mhc_hc_mix_fwd": [_P] * 16 + [_L, _P, _L, _P, _L, _L, _L, _I, _I, _F, _P],
     "mhc_add_residual_pool_fwd": [_P, _P, _P, _P, _P, _L, _L, _L, _I, _P],
     "mhc_add_residual_mix_fwd": [_P, _P, _P, _P, _P, _P, _L, _L, _L, _I, _P],
+    "mhc_counter_dropout": [_P, _P, _I, _L, _P, _L, _L, _I, _P],
+    "mhc_add_residual_dropout_fwd": [_P, _P, _P, _P, _P, _I, _L, _P, _P, _L, _L, _L, _I, _P],
+    "mhc_add_residual_dropout_bwd": [_P, _P, _P, _P, _I, _L, _P, _P, _P, _L, _P, _L, _L, _L, _I, _P],
+    "mhc_add_rms_norm_fwd": [_P, _P, _P, _I, _P, _I, _L, _P, _P, _P, _L, _L, _I, _F, _P],
+    "mhc_add_rms_norm_quant_fwd": [_P, _P, _P, _I, _P, _P, _P, _L, _I, _L, _L, _I, _F, _P],
+    "mhc_rms_norm_bwd": [_P, _P, _P, _P, _P, _I, _P, _I, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P],
+    "mhc_stream_norm_fwd": [_P, _P, _P, _I, _P, _P, _P, _L, _L, _L, _I, _F, _P],
+    "mhc_stream_norm_quant_fwd": [_P, _P, _P, _I, _P, _P, _L, _I, _L, _L, _L, _I, _F, _P],
+    "mhc_stream_norm_bwd": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _L, _I, _P],
+    "mhc_hc_mix_norm_fwd": [_P] * 9 + [_I, _F] + [_P] * 9 + [_L, _P, _L, _P, _L, _L, _L, _I, _I, _F, _P],
     "mhc_hc_mix_bwd": [_P] * 23 + [_L, _P, _P, _L, _L, _L, _I, _I, _F, _I, _I, _P],
 }
 
@@ -101,6 +112,16 @@ def call(name, stream, *args):
     return check(getattr(load(), name)(*args, stream))
 
 
+def call_on(like: torch.Tensor, name, *args):
+    """Invoke an entry point on torch's current stream of `like`'s device, with that device current."""
+    dev = like.device
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if dev.index == torch.cuda.current_device():
+        return check(getattr(_lib or load(), name)(*args, stream))
+    with torch.cuda.device(dev):
+        return check(getattr(_lib or load(), name)(*args, stream))
+
+
 def profile_start(only=None):
     """Start per-kernel timing inside the library (CUDA events around every kernel launch, or
     around the launches of the kernel named `only`)."""
@@ -139,6 +160,15 @@ def require_cuda(*tensors):
     for t in tensors:
         if not t.is_cuda:
             raise RuntimeError("mhc: tensors must live on a CUDA device (this build has no CPU path)")
+
+
+def require_same_device(like, *tensors):
+    """`like` and every tensor given (None is skipped) on one CUDA device."""
+    if not like.is_cuda:
+        raise RuntimeError("mhc: tensors must live on a CUDA device (this build has no CPU path)")
+    for t in tensors:
+        if t is not None and t.device != like.device:
+            raise RuntimeError(f"mhc: tensors must live on one CUDA device, got {like.device} and {t.device}")
 
 
 def ptr(t):

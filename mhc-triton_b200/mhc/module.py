@@ -5,13 +5,13 @@ modes and the forward contract follow the reference module (src/mhc/module.py:10
 there), so state dicts interchange with it.
 """
 
-from typing import Callable, Tuple
+from typing import Callable, Optional, Tuple
 
 import torch
 import torch.nn as nn
 
-from .ops import (add_residual_from_state, fused_add_residual, fused_dynamic_weights, fused_stream_mix,
-                  hyper_connection_mix, pooled_sums_of, sequence_mean_pool, sinkhorn_knopp, version_of)
+from .ops import (add_residual_from_state, fused_add_residual, fused_add_rms_norm, fused_dynamic_weights,
+                  fused_stream_mix, hyper_connection_mix, pooled_sums_of, sequence_mean_pool, sinkhorn_knopp, version_of)
 
 
 class HyperConnection(nn.Module):
@@ -20,6 +20,11 @@ class HyperConnection(nn.Module):
     forward(H) with H of shape (batch, seq, 4, dim) returns ``(branch_input, add_residual)``;
     run the wrapped layer on ``branch_input`` (batch, seq, dim) and call
     ``add_residual(branch_output)`` to get the updated (batch, seq, 4, dim) state.
+
+    What usually surrounds the wrapped layer runs in the same kernels on request: ``forward(H, norm_weight,
+    norm_eps)`` returns the RMS-normalised branch input (the weight belongs to the wrapped layer, None with a given
+    norm_eps: ones), and ``add_residual(out, dropout_p=p)`` drops elements of the branch output (see
+    mhc.counter_dropout for `rng` and `row_offset`; pass dropout_p=0 in evaluation).
 
     Args:
         dim: width of each stream
@@ -112,33 +117,45 @@ class HyperConnection(nn.Module):
     # The kernels are reached through ctypes, which a tracing compiler cannot see into: under
     # torch.compile the layer runs as an opaque eager call and the model around it is compiled.
     @torch.compiler.disable
-    def forward(self, H: torch.Tensor) -> Tuple[torch.Tensor, Callable[[torch.Tensor], torch.Tensor]]:
+    def forward(self, H: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, norm_eps: Optional[float] = None
+                ) -> Tuple[torch.Tensor, Callable[[torch.Tensor], torch.Tensor]]:
+        if norm_weight is not None and norm_eps is None:
+            norm_eps = 1e-6
         if self.use_fused_weights:
             lazy = not self.materialize_residual
+            fuse_norm = lazy and norm_eps is not None
             branch_input, H_residual, H_post, _, H_res = hyper_connection_mix(
                 H, self.H_pre_base, self.H_post_base, self.H_res_base, self.phi, self.alpha_pre, self.alpha_post,
                 self.alpha_res, self.sinkhorn_iters, self.eps, self.grad_sink, self.grads_ready_hook,
-                self.grad_accumulate, pooled_sums_of(H), lazy, self.grads_ready_event)
+                self.grad_accumulate, pooled_sums_of(H), lazy, self.grads_ready_event,
+                norm_weight if fuse_norm else None, norm_eps if fuse_norm else None)
+            if norm_eps is not None and not fuse_norm:
+                branch_input = fused_add_rms_norm(branch_input, None, norm_weight, norm_eps)[0]
             if lazy:
                 version = version_of(H)
 
-                def add_residual(branch_output: torch.Tensor, pool_for_next: bool = False) -> torch.Tensor:
+                def add_residual(branch_output: torch.Tensor, pool_for_next: bool = False, dropout_p: float = 0.0,
+                                 rng=None, row_offset: int = 0) -> torch.Tensor:
                     """pool_for_next=True: also accumulate the token sums the NEXT HyperConnection needs
                     for its mean-pool (pass the returned tensor to it as is)."""
                     if version_of(H) != version:
                         raise RuntimeError("H was modified in place between HyperConnection.forward and add_residual "
                                            "(set layer.materialize_residual = True if that is intended)")
-                    return add_residual_from_state(H_residual, H, H_res, branch_output, H_post, pool_for_next)
+                    return add_residual_from_state(H_residual, H, H_res, branch_output, H_post, pool_for_next,
+                                                   dropout_p, rng, row_offset)
 
                 return branch_input, add_residual
         else:
             H_post, H_pre, H_res = self._compute_weights(H)
             branch_input, H_residual = fused_stream_mix(H, H_pre, H_res)
+            if norm_eps is not None:
+                branch_input = fused_add_rms_norm(branch_input, None, norm_weight, norm_eps)[0]
 
-        def add_residual(branch_output: torch.Tensor, pool_for_next: bool = False) -> torch.Tensor:
+        def add_residual(branch_output: torch.Tensor, pool_for_next: bool = False, dropout_p: float = 0.0, rng=None,
+                         row_offset: int = 0) -> torch.Tensor:
             """pool_for_next=True: also accumulate the token sums the NEXT HyperConnection needs for its
             mean-pool, so that layer reads H once instead of twice (pass the returned tensor to it as is)."""
-            return fused_add_residual(H_residual, branch_output, H_post, pool_for_next)
+            return fused_add_residual(H_residual, branch_output, H_post, pool_for_next, dropout_p, rng, row_offset)
 
         return branch_input, add_residual
 

@@ -271,15 +271,20 @@ class SequenceShardedHyperConnection(torch.nn.Module):
             raise ValueError("sequence sharding supports fused dynamic HyperConnection layers only")
         self.layer, self.group, self.total_len = layer, process_group, total_len
 
-    def forward(self, H: torch.Tensor):
-        from .ops import add_residual_from_state
+    def forward(self, H: torch.Tensor, norm_weight: Optional[torch.Tensor] = None, norm_eps: Optional[float] = None):
+        """norm_weight / norm_eps as in the wrapped layer (tokens are normalised one by one, so nothing is exchanged)."""
+        from .ops import add_residual_from_state, fused_add_rms_norm
         l = self.layer
         total = self.total_len if self.total_len is not None else H.shape[1] * _group_size(self.group)
         branch_input, stand_in, H_post, _, H_res = _SequenceShardedMix.apply(
             H, l.H_pre_base, l.H_post_base, l.H_res_base, l.phi, l.alpha_pre, l.alpha_post, l.alpha_res,
             l.sinkhorn_iters, l.eps, self.group, total)
 
-        def add_residual(branch_output: torch.Tensor) -> torch.Tensor:
-            return add_residual_from_state(stand_in, H, H_res, branch_output, H_post)
+        if norm_weight is not None or norm_eps is not None:
+            branch_input = fused_add_rms_norm(branch_input, None, norm_weight, 1e-6 if norm_eps is None else norm_eps)[0]
+
+        def add_residual(branch_output: torch.Tensor, dropout_p: float = 0.0, rng=None, row_offset: int = 0) -> torch.Tensor:
+            """The dropout counts this rank's own tokens as rows: pass a different rng, or another row_offset, per rank."""
+            return add_residual_from_state(stand_in, H, H_res, branch_output, H_post, False, dropout_p, rng, row_offset)
 
         return branch_input, add_residual
