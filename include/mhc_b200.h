@@ -253,17 +253,18 @@ int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, const void* 
                                void* sum_out, void* q, void* scales, int64_t group, int scale_type,
                                int64_t rows, int64_t D, int dtype, float eps, mhc_stream_t stream);
 
-/* Gradients of mhc_add_rms_norm_fwd.  dsum: gradient of sum_out, or NULL.  s: sum_out (x itself where there
- * was neither residual nor dropout).  dx is also the residual's gradient; with dropout dx is the
- * gradient behind the mask and dresidual (may be NULL) the one before it.  dweight [D] of weight_dtype, or
- * NULL: a fixed-order sum over the rows. */
-int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* s, const float* rstd, const void* weight,
-                     int weight_dtype, const int64_t* rng, int drop_threshold, int64_t row_offset, void* dx,
-                     void* dresidual, void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows,
-                     int64_t D, int dtype, mhc_stream_t stream);
+/* Gradients of mhc_add_rms_norm_fwd; s is formed again from x and residual (NULL where the forward had none).
+ * dsum: gradient of sum_out, or NULL.  dx is also the residual's gradient; with dropout dx is the gradient behind
+ * the mask and dresidual (may be NULL) the one before it.  dweight [D] of weight_dtype, or NULL: a
+ * fixed-order sum over the rows.  Scratch (of MHC_OP_RMS_NORM_BWD) may be NULL where dweight is. */
+int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* x, const void* residual, const float* rstd,
+                     const void* weight, int weight_dtype, const int64_t* rng, int drop_threshold,
+                     int64_t row_offset, void* dx, void* dresidual, void* dweight, void* scratch,
+                     int64_t scratch_bytes, int64_t rows, int64_t D, int dtype, mhc_stream_t stream);
 
 /* Norm of the mixed streams in the kernel that mixes them: b = sum_n H_pre[n] H[n]; y = norm(b) * weight.
- * branch_input (b rounded to the activation type) and rstd [B, S] may be NULL.  Fuses the first half of
+ * branch_input (b rounded to the activation type; where it is written, the rounded b is what is normalised) and
+ * rstd [B, S] may be NULL.  Fuses the first half of
  * stream_mix_forward (src/mhc/_kernels.py:617-652) with the norm its caller runs on branch_input. */
 int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
                         void* branch_input, void* y, float* rstd, int64_t B, int64_t S, int64_t D, int dtype,

@@ -4,8 +4,11 @@
 //   rstd = 1 / sqrt(mean(s^2) + eps),  y = s * rstd * weight
 // y leaves in the activation type, or as e4m3 with one scale per row or per group of 32 / 64 / 128 columns.
 // Backward: with c = sum_d dy w s,  ds = rstd (dy w - s rstd^2 c / D) (+ the gradient that reached s directly),
-// dweight = sum_rows dy s rstd; dropout's mask is recomputed.  All sums, the norm and the scales are fp32; s is
-// normalised as computed, before it is rounded to the activation type for sum_out.
+// dweight = sum_rows dy s rstd; dropout's mask is recomputed.  All sums, the norm and the scales are fp32.  s is
+// normalised as computed, before it is rounded to the activation type for sum_out, and the backward forms it again
+// from x and residual instead of reading the rounded sum_out: one more tensor to read (5 instead of 4 of a bf16
+// backward's moves), but dweight keeps fp32 accuracy (from the rounded sums it is off by 1e-3).  Where the mix is
+// stored as branch_input, the stored value is what is normalised, so its backward, which reads it, is exact too.
 #include "common.cuh"
 #include "launch.h"
 #include "rng.cuh"
@@ -38,7 +41,8 @@ struct NormFwd {
 struct NormBwd {
   const void* dy;        // [rows, D]
   const void* dsum;      // [rows, D] or null: gradient that reaches s beside the norm
-  const void* s;         // [rows, D], or H [rows, 4, D]
+  const void* x;         // [rows, D], or H [rows, 4, D]
+  const void* res;       // [rows, D] or null
   const float* hpre;
   const float* rstd;     // [rows]
   const void* weight;
@@ -48,6 +52,7 @@ struct NormBwd {
   float* dw_part;        // [ctas, D] or null
   float* dpre_part;      // [B, chunks, 4] (Mix)
   int64_t items, S, D;   // items: rows (Add), batch elements x chunks (Mix)
+  int parts;             // rows of dw_part
   int64_t chunks;        // per batch element (Mix)
   int tpc;               // tokens per chunk (Mix)
   Drop drop;
@@ -126,8 +131,9 @@ template <typename T, Src SRC, bool DROP>
 __device__ __forceinline__ float src_at(const NormFwd& a, const DropKey& key, const float (&pre)[4], int64_t row, int64_t d) {
   if constexpr (SRC == Src::Mix) {
     const T* h = (const T*)a.x + row * 4 * a.D + d;
-    return ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + a.D))) + pre[2] * to_f32(__ldg(h + 2 * a.D))) +
-           pre[3] * to_f32(__ldg(h + 3 * a.D));
+    const float b = ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + a.D))) + pre[2] * to_f32(__ldg(h + 2 * a.D))) +
+                    pre[3] * to_f32(__ldg(h + 3 * a.D));
+    return a.sum_out ? to_f32(from_f32<T>(b)) : b;
   } else {
     float v[1] = {to_f32(__ldg((const T*)a.x + row * a.D + d))};
     if constexpr (DROP) drop_apply<1>(a.drop, drop_bits<1>(a.drop, key, row, d), v);
@@ -212,7 +218,7 @@ k_norm_any_bwd(NormBwd a) {
   if (dw)
     for (int64_t d = threadIdx.x; d < D; d += 256) dw[d] = 0.f;
   for (int64_t it = blockIdx.x; it < a.items; it += gridDim.x) {
-    int64_t r0 = it, r1 = it + 1;
+    int64_t r0 = it, r1 = it + 1;   // RowMap of this kernel: one row at a time
     float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (SRC == Src::Mix) {
       const int64_t b = it / a.chunks, c = it % a.chunks;
@@ -223,15 +229,9 @@ k_norm_any_bwd(NormBwd a) {
     }
     for (int64_t row = r0; row < r1; ++row) {
       const float rstd = __ldg(a.rstd + row);
-      auto s_at = [&](int64_t d) -> float {
-        if constexpr (SRC == Src::Mix) {
-          const T* h = (const T*)a.s + row * 4 * D + d;
-          return ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + D))) + pre[2] * to_f32(__ldg(h + 2 * D))) +
-                 pre[3] * to_f32(__ldg(h + 3 * D));
-        } else {
-          return to_f32(__ldg((const T*)a.s + row * D + d));
-        }
-      };
+      NormFwd f;
+      f.x = a.x; f.res = a.res; f.sum_out = nullptr; f.D = D; f.drop = a.drop;
+      auto s_at = [&](int64_t d) -> float { return src_at<T, SRC, DROP>(f, key, pre, row, d); };
       float c = 0.f, unused = 0.f;
       for (int64_t d = threadIdx.x; d < D; d += 256) {
         const float dy = to_f32(__ldg((const T*)a.dy + row * D + d)), s = s_at(d);
@@ -245,7 +245,7 @@ k_norm_any_bwd(NormBwd a) {
         const float dy = to_f32(__ldg((const T*)a.dy + row * D + d));
         float g[1] = {rstd * (dy * load_w<T>(a.weight, a.w_f32, d)) - s_at(d) * k};
         if constexpr (SRC == Src::Mix) {
-          const T* h = (const T*)a.s + row * 4 * D + d;
+          const T* h = (const T*)a.x + row * 4 * D + d;
           T* o = (T*)a.dx + row * 4 * D + d;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
@@ -265,6 +265,359 @@ k_norm_any_bwd(NormBwd a) {
     if constexpr (SRC == Src::Mix) {
       __syncthreads();
       block_reduce_store<4>(acc, a.dpre_part + it * 4, red);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ rows that divide into 16-byte packs, in registers
+// A row belongs to `tpr` threads (a multiple of 32) that own the packs t, t + tpr, ...: NP packs each, all loaded
+// before the first use and kept in registers as fp32 between the row sum and the output, so the data is read once.
+// Narrow rows share a CTA of 256 threads.  Bound by memory; the one barrier of a row is covered by the other CTAs.
+struct RowMap {
+  int tpr;   // threads per row
+  int rpc;   // rows per CTA
+  int DV;    // packs per row
+};
+
+// Row sum (and NaN-keeping maximum) over the warps of one row; sm holds 2 x 16 floats.  One barrier.
+template <bool MAX>
+__device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, const RowMap& m, int sub) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
+  if (m.tpr == 32) return;
+  const int warp = threadIdx.x >> 5, nw = m.tpr >> 5;
+  if ((threadIdx.x & 31) == 0) {
+    sm[warp] = sum;
+    if (MAX) sm[16 + warp] = mx;
+  }
+  __syncthreads();
+  float t = 0.f, x = 0.f;
+  for (int w = sub * nw; w < (sub + 1) * nw; ++w) {
+    t += sm[w];
+    if (MAX) x = max_nan(x, sm[16 + w]);
+  }
+  sum = t;
+  mx = x;
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void load_w_pack(const void* w, int w_f32, int col, float (&o)[V]) {
+  if (!w) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = 1.f;
+  } else if (w_f32) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>((const float*)w + col + e));
+      o[e] = f.x; o[e + 1] = f.y; o[e + 2] = f.z; o[e + 3] = f.w;
+    }
+  } else {
+    RawPack<T, V> r;
+    r.w = __ldg(reinterpret_cast<const uint4*>((const T*)w + col));
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] = raw_get<V>(r, e);
+  }
+}
+
+template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], float inv) {
+  uint32_t w[V / 4];
+#pragma unroll
+  for (int i = 0; i < V / 4; ++i)
+    w[i] = (uint32_t)e4m3x2(y[4 * i] * inv, y[4 * i + 1] * inv) |
+           ((uint32_t)e4m3x2(y[4 * i + 2] * inv, y[4 * i + 3] * inv) << 16);
+  if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+  else *reinterpret_cast<uint32_t*>(p) = w[0];
+}
+
+template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
+__global__ void __launch_bounds__(512)
+k_norm_fwd(NormFwd a, RowMap m) {
+  pdl_prologue();
+  __shared__ float sm[32];
+  const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
+  const int64_t row = (int64_t)blockIdx.x * m.rpc + sub, D = a.D;
+  const bool live = row < a.rows;
+  constexpr int NS = SRC == Src::Mix ? 4 : 2;
+  RawPack<T, V> raw[NP][NS];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int p = t + k * m.tpr;
+#pragma unroll
+    for (int n = 0; n < NS; ++n) raw[k][n].w = make_uint4(0, 0, 0, 0);
+    if (live && p < m.DV) {
+      if constexpr (SRC == Src::Mix) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) raw[k][n] = ld_raw<T, V>((const T*)a.x + (row * 4 + n) * D + p * V);
+      } else {
+        raw[k][0] = ld_raw<T, V>((const T*)a.x + row * D + p * V);
+        if (a.res) raw[k][1] = ld_raw<T, V>((const T*)a.res + row * D + p * V);
+      }
+    }
+  }
+  float pre[4] = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (SRC == Src::Mix) {
+    if (live) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + row / a.S * 4 + n);
+    }
+  }
+  float w[NP][V];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int p = t + k * m.tpr;
+    if (p < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, p * V, w[k]);
+    else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) w[k][e] = 0.f;
+    }
+  }
+  DropKey key{};
+  if constexpr (DROP) key = drop_key(a.drop);
+  float v[NP][V], ss = 0.f, mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int p = t + k * m.tpr;
+    const bool ok = live && p < m.DV;
+    if constexpr (SRC == Src::Mix) {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        v[k][e] = ((pre[0] * raw_get<V>(raw[k][0], e) + pre[1] * raw_get<V>(raw[k][1], e)) + pre[2] * raw_get<V>(raw[k][2], e)) +
+                  pre[3] * raw_get<V>(raw[k][3], e);
+      if (a.sum_out && ok) PackIO<T, V>::store_round((T*)a.sum_out + row * D + p * V, v[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k][e] = raw_get<V>(raw[k][0], e);
+      if constexpr (DROP) {
+        if (ok) drop_apply<V>(a.drop, drop_bits<V>(a.drop, key, row, p * V), v[k]);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(raw[k][1], e);
+      if (a.sum_out && ok) PackIO<T, V>::store((T*)a.sum_out + row * D + p * V, v[k]);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      ss = fmaf(v[k][e], v[k][e], ss);
+      if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v[k][e] * w[k][e]));
+    }
+  }
+  row_sum_max<OUT == Out::RowScale>(ss, mx, sm, m, sub);
+  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + a.eps));
+  if (a.rstd && live && t == 0) a.rstd[row] = rstd;
+  Scale sc{};
+  if constexpr (OUT == Out::RowScale) {
+    sc = make_scale(mx * rstd, a.e8m0);
+    if (live && t == 0) store_scale(a.scales, row, sc, a.e8m0);
+  }
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int p = t + k * m.tpr;
+    const bool ok = live && p < m.DV;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * rstd * w[k][e];
+    if constexpr (OUT == Out::GroupScale) {   // group / V consecutive packs = consecutive lanes
+      float g = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) g = max_nan(g, fabsf(v[k][e]));
+      const int lanes = a.group / V;
+      for (int o = lanes >> 1; o > 0; o >>= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
+      sc = make_scale(g, a.e8m0);
+      if (ok && (p & (lanes - 1)) == 0) store_scale(a.scales, row * ((D + a.group - 1) / a.group) + p / lanes, sc, a.e8m0);
+    }
+    if (ok) {
+      if constexpr (OUT == Out::Plain) PackIO<T, V>::store((T*)a.y + row * D + p * V, v[k]);
+      else store_e4m3<V>((uint8_t*)a.y + row * D + p * V, v[k], sc.inv);
+    }
+  }
+}
+
+// Backward: persistent CTAs, so that the threads, which own the same columns in every row, keep the weight and
+// dweight's running sums in registers.  While a row is worked on the next one's packs are already on the way (PIPE).
+// An item is a row of rpc (Add) or a chunk of a batch element's tokens (Mix), walked rpc abreast.
+template <typename T, int V, int NP, Src SRC, bool DROP, bool PIPE>
+__global__ void __launch_bounds__(512)
+k_norm_bwd(NormBwd a, RowMap m) {
+  pdl_prologue();
+  __shared__ float sm[2][32];
+  __shared__ float red[16 * 4];
+  constexpr int NS = SRC == Src::Mix ? 5 : 4;   // Mix: dy, H[0..3]; Add: dy, x, residual, dsum
+  struct RowRaw {
+    RawPack<T, V> p[NP][NS];
+    float rstd;
+  };
+  const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
+  const int64_t D = a.D;
+  DropKey key{};
+  if constexpr (DROP) key = drop_key(a.drop);
+  float w[NP][V], dw[NP][V];
+#pragma unroll
+  for (int k = 0; k < NP; ++k) {
+    const int p = t + k * m.tpr;
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[k][e] = w[k][e] = 0.f;
+    if (p < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, p * V, w[k]);
+  }
+  const float inv_D = __fdiv_rn(1.f, (float)D);
+
+  // where this CTA is: rows base .. base + rpc - 1 of the item, the item's end, the item
+  struct Pos { int64_t item, base, end; };
+  auto enter = [&](Pos& q) {   // first rows of q.item
+    if (q.item >= a.items) return;
+    if constexpr (SRC == Src::Mix) {
+      const int64_t b = q.item / a.chunks, c = q.item - b * a.chunks;
+      q.base = b * a.S + c * a.tpc;
+      q.end = min(q.base + a.tpc, (b + 1) * a.S);
+    } else {
+      q.base = q.item * m.rpc;
+      q.end = min(q.base + m.rpc, a.S);
+    }
+  };
+  auto next = [&](Pos q) -> Pos {
+    q.base += m.rpc;
+    if (q.base >= q.end) {
+      q.item += gridDim.x;
+      enter(q);
+    }
+    return q;
+  };
+  auto load = [&](RowRaw& r, const Pos& q) {
+    const int64_t row = q.base + sub;
+    const bool live = q.item < a.items && row < q.end;
+    r.rstd = live ? __ldg(a.rstd + row) : 0.f;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int p = t + k * m.tpr;
+#pragma unroll
+      for (int n = 0; n < NS; ++n) r.p[k][n].w = make_uint4(0, 0, 0, 0);
+      if (live && p < m.DV) {
+        r.p[k][0] = ld_raw<T, V>((const T*)a.dy + row * D + p * V);
+        if constexpr (SRC == Src::Mix) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) r.p[k][1 + n] = ld_raw<T, V>((const T*)a.x + (row * 4 + n) * D + p * V);
+        } else {
+          r.p[k][1] = ld_raw<T, V>((const T*)a.x + row * D + p * V);
+          if (a.res) r.p[k][2] = ld_raw<T, V>((const T*)a.res + row * D + p * V);
+          if (a.dsum) r.p[k][3] = ld_raw<T, V>((const T*)a.dsum + row * D + p * V);
+        }
+      }
+    }
+  };
+  float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  int64_t pre_of = -1;
+  int parity = 0;
+  auto work = [&](const RowRaw& r, const Pos& q, bool last_of_item) {
+    const int64_t row = q.base + sub;
+    const bool live = row < q.end;
+    if constexpr (SRC == Src::Mix) {
+      if (q.item != pre_of) {
+        pre_of = q.item;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + q.item / a.chunks * 4 + n);
+      }
+    }
+    float s[NP][V], c = 0.f, unused = 0.f;
+    DropBits<V> bits[DROP ? NP : 1];
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int p = t + k * m.tpr;
+      if constexpr (SRC == Src::Mix) {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          s[k][e] = ((pre[0] * raw_get<V>(r.p[k][1], e) + pre[1] * raw_get<V>(r.p[k][2], e)) +
+                     pre[2] * raw_get<V>(r.p[k][3], e)) + pre[3] * raw_get<V>(r.p[k][4], e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(r.p[k][1], e);
+        if constexpr (DROP) {
+          bits[k] = drop_bits<V>(a.drop, key, row, p * V);
+          drop_apply<V>(a.drop, bits[k], s[k]);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r.p[k][2], e);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float dy = raw_get<V>(r.p[k][0], e);
+        c = fmaf(dy * w[k][e], s[k][e], c);
+        dw[k][e] = fmaf(dy, s[k][e] * r.rstd, dw[k][e]);
+      }
+    }
+    row_sum_max<false>(c, unused, sm[parity], m, sub);
+    parity ^= 1;   // the next row's sums go to the other half: nobody can still be reading it
+    const float kk = c * r.rstd * r.rstd * r.rstd * inv_D;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int p = t + k * m.tpr;
+      const bool ok = live && p < m.DV;
+      float g[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = r.rstd * (raw_get<V>(r.p[k][0], e) * w[k][e]) - s[k][e] * kk;
+      if constexpr (SRC == Src::Mix) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          float o[V];
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            acc[n] = fmaf(g[e], raw_get<V>(r.p[k][1 + n], e), acc[n]);
+            o[e] = pre[n] * g[e];
+          }
+          if (ok) PackIO<T, V>::store((T*)a.dx + (row * 4 + n) * D + p * V, o);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) g[e] += raw_get<V>(r.p[k][3], e);
+        if constexpr (DROP) {
+          if (ok && a.dres) PackIO<T, V>::store((T*)a.dres + row * D + p * V, g);
+          drop_apply<V>(a.drop, bits[k], g);
+        }
+        if (ok) PackIO<T, V>::store((T*)a.dx + row * D + p * V, g);
+      }
+    }
+    if constexpr (SRC == Src::Mix) {
+      if (last_of_item) {
+        __syncthreads();   // the previous item's readers of red are done
+        block_reduce_store<4>(acc, a.dpre_part + q.item * 4, red);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[n] = 0.f;
+      }
+    }
+  };
+
+  Pos q{(int64_t)blockIdx.x, 0, 0};
+  enter(q);
+  if constexpr (PIPE) {
+    RowRaw ra, rb;
+    load(ra, q);
+    while (q.item < a.items) {
+      const Pos q2 = next(q);
+      load(rb, q2);
+      work(ra, q, q2.item != q.item);
+      if (q2.item >= a.items) break;
+      q = next(q2);
+      load(ra, q);
+      work(rb, q2, q.item != q2.item);
+    }
+  } else {
+    RowRaw ra;
+    while (q.item < a.items) {
+      load(ra, q);
+      const Pos q2 = next(q);
+      work(ra, q, q2.item != q.item);
+      q = q2;
+    }
+  }
+  if (a.dw_part) {
+    float* o = a.dw_part + ((int64_t)blockIdx.x * m.rpc + sub) * D;
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int p = t + k * m.tpr;
+      if (p < m.DV) {
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+          *reinterpret_cast<float4*>(o + p * V + e) = make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]);
+      }
     }
   }
 }
@@ -291,17 +644,42 @@ k_norm_dweight(const float* __restrict__ part, int64_t n, int64_t D, T* __restri
 }
 
 // --------------------------------------------------------------------------------------------------- host side
-// CTAs of the backward: enough to fill the device twice over; each leaves one row of dweight partial sums.
-static int64_t bwd_ctas(int64_t items) {
-  const int64_t most = 2 * (int64_t)sm_count();
+// The backward's persistent grid: two CTAs of 256 threads per SM (its registers allow no more), one of the wider ones.
+// Every row a CTA walks abreast leaves one row of dweight partial sums.
+static int64_t bwd_ctas(int64_t items, int threads) {
+  const int64_t most = (threads > 256 ? 1 : 2) * (int64_t)sm_count();
   return items < most ? items : most;
 }
-constexpr int kMixTpc = 8;  // tokens per chunk of the stream-norm backward
-static int64_t mix_chunks(int64_t S) { return (S + kMixTpc - 1) / kMixTpc; }
+// Tokens per chunk of the stream-norm backward: as many chunks per batch element as fill the device's CTAs once (so any
+// number of batch elements fills them evenly), but four rounds of rpc tokens at least, since a chunk ends with a
+// reduction.  A function of the sequence and the width only: a batch element sums in the same order in any batch.
+static int64_t mix_tpc(int64_t S, int rpc) {
+  const int64_t even = (S + 2 * sm_count() - 1) / (2 * sm_count()), least = S < 4 * rpc ? S : 4 * rpc;
+  const int64_t n = even > least ? even : least;
+  return n > 0 ? n : 1;
+}
+static int64_t mix_chunks(int64_t S, int rpc) { return (S + mix_tpc(S, rpc) - 1) / mix_tpc(S, rpc); }
 
-int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D) { return bwd_ctas(rows) * D * (int64_t)sizeof(float); }
+// Threads and rows per CTA for rows of D elements in packs of V: `np` packs per thread.
+static RowMap row_map(int64_t D, int V, int np) {
+  RowMap m;
+  m.DV = (int)(D / V);
+  m.tpr = ((m.DV + np - 1) / np + 31) / 32 * 32;
+  m.rpc = m.tpr <= 128 ? 256 / m.tpr : 1;
+  return m;
+}
+// Packs per thread of the register kernels: 2 up to 1024 packs per row, 4 up to 2048; 0: the row does not fit.
+static int packs_per_thread(int64_t D, int V) { return D / V <= 1024 ? 2 : D / V <= 2048 ? 4 : 0; }
+
+// Scratch: at most two rows' worth of partial sums per SM and row walked abreast (rpc <= 8, and then D <= 512), plus the
+// chunks' dH_pre sums.
+static int64_t dw_rows(int64_t D) { return 2 * (int64_t)sm_count() * (D <= 512 ? 8 : D <= 1024 ? 4 : D <= 2048 ? 2 : 1); }
+int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D) {
+  const int64_t n = dw_rows(D);
+  return ((rows < n ? (rows + 7) / 8 * 8 : n) * D + 4) * (int64_t)sizeof(float);
+}
 int64_t stream_norm_bwd_scratch_bytes(int64_t B, int64_t S, int64_t D) {
-  return (bwd_ctas(B * mix_chunks(S)) * D + B * mix_chunks(S) * 4) * (int64_t)sizeof(float);
+  return (dw_rows(D) * D + B * mix_chunks(S, 1) * 4 + 4) * (int64_t)sizeof(float);
 }
 
 #define MHC_TYPE_DISPATCH(dtype, CALL)                             \
@@ -331,14 +709,48 @@ static int check_quant(const char* what, int64_t group, int scale_type) {
 template <Src SRC, bool DROP, Out OUT>
 static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_t st) {
   ProfScope ps(SRC == Src::Mix ? "k_stream_norm_fwd" : "k_rms_norm_fwd", st);
-  MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_fwd<T, SRC, DROP, OUT>, (unsigned)a.rows, 256, 0, st, a)));
+  const int vec = pick_vec(dtype, a.D, {a.x, a.res, a.weight, a.sum_out, a.y});
+  const int np = vec > 1 ? packs_per_thread(a.D, vec) : 0;
+  if (np == 0) {
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_fwd<T, SRC, DROP, OUT>, (unsigned)a.rows, 256, 0, st, a)));
+    return check_launch(what);
+  }
+  const RowMap m = row_map(a.D, vec, np);
+  const unsigned grid = (unsigned)((a.rows + m.rpc - 1) / m.rpc), block = (unsigned)(m.tpr * m.rpc);
+  if (np == 2) MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, vec_width<T>::value, 2, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
+  else MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, vec_width<T>::value, 4, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
   return check_launch(what);
 }
 
+// Fills in what depends on the kernel chosen (items, chunks, partial rows) and launches; a.items are rows (Add) or
+// batch elements (Mix) on entry.
 template <Src SRC, bool DROP>
-static int launch_bwd(const char* what, const NormBwd& a, int64_t ctas, int dtype, cudaStream_t st) {
+static int launch_bwd(const char* what, NormBwd& a, float* scratch, int dtype, cudaStream_t st) {
   ProfScope ps(SRC == Src::Mix ? "k_stream_norm_bwd" : "k_rms_norm_bwd", st);
-  MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_bwd<T, SRC, DROP>, (unsigned)ctas, 256, 0, st, a)));
+  const int vec = pick_vec(dtype, a.D, {a.dy, a.dsum, a.x, a.res, a.weight, a.dx, a.dres});
+  const int np = vec > 1 ? packs_per_thread(a.D, vec) : 0;
+  RowMap m{256, 1, 0};
+  if (np) m = row_map(a.D, vec, np);
+  if constexpr (SRC == Src::Mix) {
+    a.tpc = (int)mix_tpc(a.S, m.rpc);
+    a.chunks = mix_chunks(a.S, m.rpc);
+    a.items *= a.chunks;
+  } else {
+    a.S = a.items;
+    a.items = (a.S + m.rpc - 1) / m.rpc;
+  }
+  const int threads = m.tpr * m.rpc;
+  const int64_t ctas = bwd_ctas(a.items, threads);
+  a.parts = (int)(ctas * m.rpc);
+  scratch = (float*)(((uintptr_t)scratch + 15) & ~(uintptr_t)15);
+  if (a.dw_part) { a.dw_part = scratch; scratch += a.parts * a.D; }
+  a.dpre_part = scratch;
+  if (np == 0)
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_bwd<T, SRC, DROP>, (unsigned)ctas, 256, 0, st, a)));
+  else if (np == 2)
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, vec_width<T>::value, 2, SRC, DROP, true>, (unsigned)ctas, threads, 0, st, a, m)));
+  else
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, vec_width<T>::value, 4, SRC, DROP, false>, (unsigned)ctas, threads, 0, st, a, m)));
   return check_launch(what);
 }
 
@@ -398,8 +810,8 @@ extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, c
                : launch_fwd<Src::Add, false, Out::RowScale>(what, a, dtype, st);
 }
 
-extern "C" int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* s, const float* rstd, const void* weight,
-                                int weight_dtype, const int64_t* rng, int drop_threshold, int64_t row_offset, void* dx,
+extern "C" int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* x, const void* residual, const float* rstd,
+                                const void* weight, int weight_dtype, const int64_t* rng, int drop_threshold, int64_t row_offset, void* dx,
                                 void* dresidual, void* dweight, void* scratch, int64_t scratch_bytes, int64_t rows,
                                 int64_t D, int dtype, mhc_stream_t stream) {
   const char* what = "rms_norm_bwd";
@@ -419,15 +831,15 @@ extern "C" int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* s,
   if (dweight && scratch_bytes < rms_norm_bwd_scratch_bytes(rows, D))
     return fail(MHC_ERR_SCRATCH_TOO_SMALL, "%s: scratch %lld < %lld bytes", what, (long long)scratch_bytes,
                 (long long)rms_norm_bwd_scratch_bytes(rows, D));
-  if (!dy || !s || !rstd || !dx || (dweight && !scratch)) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
+  if (!dy || !x || !rstd || !dx || (dweight && !scratch)) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   if (!is_aligned_to(scratch, 4)) return fail(MHC_ERR_MISALIGNED, "%s: scratch must be 4-byte aligned", what);
   if (!drop && dresidual) return fail(MHC_ERR_BAD_ARGUMENT, "%s: without dropout the residual's gradient is dx", what);
-  a.dy = dy; a.dsum = dsum; a.s = s; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dx;
-  a.dres = dresidual; a.dw_part = dweight ? (float*)scratch : nullptr; a.items = rows; a.S = 1; a.D = D;
-  const int64_t ctas = bwd_ctas(rows);
-  if (int e = drop ? launch_bwd<Src::Add, true>(what, a, ctas, dtype, st) : launch_bwd<Src::Add, false>(what, a, ctas, dtype, st))
+  a.dy = dy; a.dsum = dsum; a.x = x; a.res = residual; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32;
+  a.dx = dx; a.dres = dresidual; a.dw_part = dweight ? (float*)scratch : nullptr; a.items = rows; a.D = D;
+  if (int e = drop ? launch_bwd<Src::Add, true>(what, a, (float*)scratch, dtype, st)
+                   : launch_bwd<Src::Add, false>(what, a, (float*)scratch, dtype, st))
     return e;
-  return dweight ? finish_dweight(what, a.dw_part, ctas, D, dweight, weight_dtype, st) : MHC_OK;
+  return dweight ? finish_dweight(what, a.dw_part, a.parts, D, dweight, weight_dtype, st) : MHC_OK;
 }
 
 extern "C" int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
@@ -484,12 +896,9 @@ extern "C" int mhc_stream_norm_bwd(const void* dy, const void* H, const float* H
   if (!dy || !H || !H_pre || !rstd || !dH || !dH_pre || !scratch) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   if (!is_aligned_to(scratch, 4)) return fail(MHC_ERR_MISALIGNED, "%s: scratch must be 4-byte aligned", what);
   NormBwd a{};
-  a.dy = dy; a.s = H; a.hpre = H_pre; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dH;
-  a.chunks = mix_chunks(S); a.tpc = kMixTpc; a.items = B * a.chunks; a.S = S; a.D = D;
-  const int64_t ctas = bwd_ctas(a.items);
-  a.dpre_part = (float*)scratch;
-  a.dw_part = dweight ? a.dpre_part + a.items * 4 : nullptr;
-  if (int e = launch_bwd<Src::Mix, false>(what, a, ctas, dtype, st)) return e;
+  a.dy = dy; a.x = H; a.hpre = H_pre; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dH;
+  a.dw_part = dweight ? (float*)scratch : nullptr; a.items = B; a.S = S; a.D = D;
+  if (int e = launch_bwd<Src::Mix, false>(what, a, (float*)scratch, dtype, st)) return e;
   if (int e = reduce_partials_impl(a.dpre_part, B, a.chunks, 4, dH_pre, st, what)) return e;
-  return dweight ? finish_dweight(what, a.dw_part, ctas, D, dweight, weight_dtype, st) : MHC_OK;
+  return dweight ? finish_dweight(what, a.dw_part, a.parts, D, dweight, weight_dtype, st) : MHC_OK;
 }

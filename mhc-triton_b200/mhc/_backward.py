@@ -206,26 +206,29 @@ def add_residual_dropout_backward(dH_new, branch_output, H_post, rng, threshold:
     return dH_new, d_bo, dH_post
 
 
-def rms_norm_backward(dy, dsum, s, rstd, weight=None, rng=None, threshold: int = 0, row_offset: int = 0,
+def rms_norm_backward(dy, dsum, x, residual, rstd, weight=None, rng=None, threshold: int = 0, row_offset: int = 0,
                       want_dresidual: bool = False, want_dweight: bool = True):
     """(dx, dresidual, dweight) of add_rms_norm_forward from the gradients of y and of s (dsum, or None).  Without
     dropout dresidual IS dx; dweight has the weight's type (None if not wanted)."""
-    D = s.shape[-1]
-    _check(dy.shape == s.shape and (dsum is None or dsum.shape == s.shape) and rstd.numel() == _rows(s), "shape mismatch")
-    L.require_same_device(s, dy, dsum, rstd, weight, rng)
-    s = s.contiguous()
-    dy = dy.to(s.dtype).contiguous()
-    dsum = None if dsum is None else dsum.to(s.dtype).contiguous()
-    w, wcode = _norm_weight(weight, s, D)
-    dx = torch.empty_like(s)
-    dres = torch.empty_like(s) if threshold and want_dresidual else None
+    D = x.shape[-1]
+    rows = _rows(x)
+    _check(dy.shape == x.shape and (dsum is None or dsum.shape == x.shape) and
+           (residual is None or residual.shape == x.shape) and rstd.numel() == rows, "shape mismatch")
+    L.require_same_device(x, dy, dsum, residual, rstd, weight, rng)
+    x = x.contiguous()
+    residual = None if residual is None else residual.to(x.dtype).contiguous()
+    dy = dy.to(x.dtype).contiguous()
+    dsum = None if dsum is None else dsum.to(x.dtype).contiguous()
+    w, wcode = _norm_weight(weight, x, D)
+    dx = torch.empty_like(x)
+    dres = torch.empty_like(x) if threshold and want_dresidual else None
     dw, buf, nbytes = None, None, 0
     if want_dweight and w is not None:
         dw = torch.empty_like(w)
-        buf, nbytes = L.scratch(L.OP_RMS_NORM_BWD, 0, _rows(s), D, s)
-    L.call_on(s, "mhc_rms_norm_bwd", dy.data_ptr(), L.ptr(dsum), s.data_ptr(), rstd.data_ptr(), L.ptr(w), wcode,
-              L.ptr(rng), threshold, row_offset, dx.data_ptr(), L.ptr(dres), L.ptr(dw), L.ptr(buf), nbytes, _rows(s), D,
-              L.dtype_code(s))
+        buf, nbytes = L.scratch(L.OP_RMS_NORM_BWD, 0, rows, D, x)
+    L.call_on(x, "mhc_rms_norm_bwd", dy.data_ptr(), L.ptr(dsum), x.data_ptr(), L.ptr(residual), rstd.data_ptr(), L.ptr(w),
+              wcode, L.ptr(rng), threshold, row_offset, dx.data_ptr(), L.ptr(dres), L.ptr(dw), L.ptr(buf), nbytes, rows, D,
+              L.dtype_code(x))
     if dw is not None and dw.dtype != weight.dtype:
         dw = dw.to(weight.dtype)
     return dx, (dres if threshold else dx), dw

@@ -47,7 +47,7 @@ _PROTOTYPES = {
     "mhc_add_residual_dropout_bwd": [_P, _P, _P, _P, _I, _L, _P, _P, _P, _L, _P, _L, _L, _L, _I, _P],
     "mhc_add_rms_norm_fwd": [_P, _P, _P, _I, _P, _I, _L, _P, _P, _P, _L, _L, _I, _F, _P],
     "mhc_add_rms_norm_quant_fwd": [_P, _P, _P, _I, _P, _P, _P, _L, _I, _L, _L, _I, _F, _P],
-    "mhc_rms_norm_bwd": [_P, _P, _P, _P, _P, _I, _P, _I, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P],
+    "mhc_rms_norm_bwd": [_P, _P, _P, _P, _P, _P, _I, _P, _I, _L, _P, _P, _P, _P, _L, _L, _L, _I, _P],
     "mhc_stream_norm_fwd": [_P, _P, _P, _I, _P, _P, _P, _L, _L, _L, _I, _F, _P],
     "mhc_stream_norm_quant_fwd": [_P, _P, _P, _I, _P, _P, _L, _I, _L, _L, _L, _I, _F, _P],
     "mhc_stream_norm_bwd": [_P, _P, _P, _P, _P, _I, _P, _P, _P, _P, _L, _L, _L, _L, _I, _P],

@@ -210,7 +210,7 @@ class _HyperConnectionMix(torch.autograd.Function):
         d_norm_weight = None
         if ctx.has_norm:   # the gradient of the normalised branch input -> that of the mix
             mixed, rstd, norm_weight = ctx.saved_tensors[12:]
-            d_branch_input, _, d_norm_weight = rms_norm_backward(d_branch_input, None, mixed, rstd, norm_weight,
+            d_branch_input, _, d_norm_weight = rms_norm_backward(d_branch_input, None, mixed, None, rstd, norm_weight,
                                                                  want_dweight=ctx.needs_input_grad[16])
         if dH_residual is None:
             dH_residual = torch.zeros_like(H)
@@ -276,9 +276,8 @@ class _AddRmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, eps, rng, threshold, row_offset):
         y, s, rstd = add_rms_norm_forward(x, residual, weight, eps, rng, threshold, row_offset)
-        ctx.save_for_backward(s, rstd, weight, rng)
+        ctx.save_for_backward(x, residual, rstd, weight, rng)   # s is formed again: rounded, it would cost dweight its accuracy
         ctx.threshold, ctx.row_offset = threshold, row_offset
-        ctx.residual_dtype = None if residual is None else residual.dtype
         ctx.set_materialize_grads(False)
         return (y, s) if residual is not None or threshold else y
 
@@ -287,13 +286,13 @@ class _AddRmsNorm(torch.autograd.Function):
     def backward(ctx, dy, ds=None):
         if dy is None and ds is None:
             return (None,) * 7
-        s, rstd, weight, rng = ctx.saved_tensors
+        x, residual, rstd, weight, rng = ctx.saved_tensors
         if dy is None:
-            dy = torch.zeros_like(s)
+            dy = torch.zeros_like(x)
         need_x, need_res, need_w = ctx.needs_input_grad[:3]
-        dx, dres, dw = rms_norm_backward(dy, ds, s, rstd, weight, rng, ctx.threshold, ctx.row_offset,
+        dx, dres, dw = rms_norm_backward(dy, ds, x, residual, rstd, weight, rng, ctx.threshold, ctx.row_offset,
                                          want_dresidual=need_res, want_dweight=need_w)
-        return (dx if need_x else None, dres.to(ctx.residual_dtype) if need_res else None, dw, None, None, None, None)
+        return (dx if need_x else None, dres.to(residual.dtype) if need_res else None, dw, None, None, None, None)
 
 
 class _FusedStreamNorm(torch.autograd.Function):

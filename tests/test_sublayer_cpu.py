@@ -75,11 +75,11 @@ def test_c_refusals_of_the_norm():
     assert q(None, None, None, 0, None, None, None, 32, 2, 4, 16, 0, 1e-6, None) == 4           # scale type
     assert q(None, None, None, 0, None, None, None, 32, 1, 4, 16, 0, 1e-6, None) == 1
     b = lib.mhc_rms_norm_bwd
-    assert b(None, None, None, None, None, 0, None, 0, 0, None, None, 64, None, 3, 4, 16, 0, None) == 5   # scratch
-    assert b(None, None, None, None, None, 0, None, 0, 0, None, None, None, None, 0, 4, 16, 0, None) == 1
+    assert b(None, None, None, None, None, None, 0, None, 0, 0, None, None, 64, None, 3, 4, 16, 0, None) == 5   # scratch
+    assert b(None, None, None, None, None, None, 0, None, 0, 0, None, None, None, None, 0, 4, 16, 0, None) == 1
     buf = ctypes.create_string_buffer(64)
     p = (ctypes.addressof(buf) + 15) & ~15
-    assert b(p, None, p, p, None, 0, None, 0, 0, p, p, None, None, 0, 4, 16, 0, None) == 4      # dresidual without dropout
+    assert b(p, None, p, None, p, None, 0, None, 0, 0, p, p, None, None, 0, 4, 16, 0, None) == 4      # dresidual without dropout
     s = lib.mhc_stream_norm_fwd
     assert s(None, None, None, 0, None, None, None, 2, 3, 16, 0, 1e-6, None) == 1
     assert s(None, None, None, 0, None, None, None, 1 << 20, 1 << 20, 16, 0, 1e-6, None) == 2   # more tokens than a grid has CTAs
