@@ -6,32 +6,65 @@
 
 namespace mhc {
 
-// One thread per pack of V columns (V > 1), or per group of 8 columns read one by one (V = 1: rows that do not
-// divide into 16-byte packs).
+// A thread owns one group of columns (a 16-byte pack; for V = 1, rows that do not divide into packs, 8 columns read one
+// by one) and walks kDropRows rows: the column's part of the generator is computed once and all loads are
+// issued before the first use.
+#ifndef MHC_DROP_ROWS
+#define MHC_DROP_ROWS 4
+#endif
+constexpr int kDropRows = MHC_DROP_ROWS;
+struct DropGeo {
+  int64_t rows, D;
+  int groups;   // column groups of a row
+  int cols;     // column groups per CTA (threads abreast in a row)
+  int sub;      // rows abreast
+  int CG;       // CTAs side by side in a row
+};
+
 template <typename T, int V>
 __global__ void __launch_bounds__(256)
-k_counter_dropout(const T* __restrict__ x, T* __restrict__ y, int64_t items, uint32_t per_row, int64_t D, Drop drop) {
+k_counter_dropout(const T* __restrict__ x, T* __restrict__ y, DropGeo g, Drop drop) {
   pdl_prologue();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= items) return;
-  const DropKey key = drop_key(drop);
-  const int64_t row = i <= 0xffffffffLL ? (int64_t)((uint32_t)i / per_row) : i / per_row;
-  const int64_t pos = i - row * per_row;
+  const int64_t chunk = g.CG == 1 ? blockIdx.x : blockIdx.x / g.CG;
+  const int cg = g.CG == 1 ? 0 : (int)(blockIdx.x - chunk * g.CG);
+  const int s = threadIdx.x / g.cols, pos = cg * g.cols + threadIdx.x - s * g.cols;
+  if (pos >= g.groups) return;
+  const int64_t row0 = chunk * (kDropRows * g.sub) + s, step = g.sub;
+  const DropSeed seed = drop_seed(drop);
   if constexpr (V > 1) {
-    float v[V];
-    const int64_t col = pos * V;
-    PackIO<T, V>::load(x + row * D + col, v);
-    drop_apply<V>(drop, drop_bits<V>(drop, key, row, col), v);
-    PackIO<T, V>::store(y + row * D + col, v);
+    const int64_t col = (int64_t)pos * V;
+    RawPack<T, V> raw[kDropRows];
+#pragma unroll
+    for (int r = 0; r < kDropRows; ++r)
+      if (row0 + r * step < g.rows) raw[r] = ld_raw<T, V>(x + (row0 + r * step) * g.D + col);
+    const DropCol dc = drop_col(seed, (uint32_t)(col >> 3));
+#pragma unroll
+    for (int r = 0; r < kDropRows; ++r) {
+      const int64_t row = row0 + r * step;
+      if (row < g.rows) {
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = raw_get<V>(raw[r], e);
+        drop_apply<V>(drop, drop_bits<V>(seed, dc, drop_row(drop, seed, row), col), v);
+        PackIO<T, V>::store(y + row * g.D + col, v);
+      }
+    }
   } else {
-    const int64_t col = pos * 8, base = row * D + col;
-    float v[8];
+    const int64_t col = (int64_t)pos * 8;
+    const DropCol dc = drop_col(seed, (uint32_t)pos);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = col + e < D ? to_f32(x[base + e]) : 0.f;
-    drop_apply<8>(drop, drop_bits<8>(drop, key, row, col), v);
+    for (int r = 0; r < kDropRows; ++r) {
+      const int64_t row = row0 + r * step, base = row * g.D + col;
+      if (row < g.rows) {
+        float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (col + e < D) y[base + e] = from_f32<T>(v[e]);
+        for (int e = 0; e < 8; ++e) v[e] = col + e < g.D ? to_f32(x[base + e]) : 0.f;
+        drop_apply<8>(drop, drop_bits<8>(seed, dc, drop_row(drop, seed, row), col), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < g.D) y[base + e] = from_f32<T>(v[e]);
+      }
+    }
   }
 }
 
@@ -63,13 +96,20 @@ extern "C" int mhc_counter_dropout(const void* x, const int64_t* rng, int drop_t
   if (rows == 0 || D == 0) return MHC_OK;
   if (!x || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   const int vec = pick_vec(dtype, D, {x, y});
-  const int64_t per_row = vec > 1 ? D / vec : (D + 7) / 8, items = rows * per_row, grid = (items + 255) / 256;
+  DropGeo g;
+  g.rows = rows;
+  g.D = D;
+  g.groups = (int)(vec > 1 ? D / vec : (D + 7) / 8);
+  g.cols = g.groups >= 256 ? 256 : (g.groups + 31) / 32 * 32;
+  g.sub = 256 / g.cols;
+  g.CG = (g.groups + g.cols - 1) / g.cols;
+  const int64_t grid = (rows + kDropRows * g.sub - 1) / (kDropRows * g.sub) * g.CG;
   if (grid > kMaxGridItems) return fail(MHC_ERR_BAD_SHAPE, "%s: too many work items (%lld)", what, (long long)grid);
   cudaStream_t st = (cudaStream_t)stream;
   {
     ProfScope ps("k_counter_dropout", st);
-    MHC_DISPATCH(dtype, vec, (launch_k(k_counter_dropout<T, V>, (unsigned)grid, 256, 0, st, (const T*)x, (T*)y, items,
-                                       (uint32_t)per_row, D, drop)));
+    MHC_DISPATCH(dtype, vec, (launch_k(k_counter_dropout<T, V>, (unsigned)grid, (unsigned)(g.cols * g.sub), 0, st,
+                                       (const T*)x, (T*)y, g, drop)));
   }
   return check_launch(what);
 }

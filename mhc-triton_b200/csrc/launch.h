@@ -140,7 +140,6 @@ inline int64_t rows_of(int64_t B, int64_t S) {  // B * S, or a count no check ac
 int make_drop(const char* what, const int64_t* rng, int threshold, int64_t row_offset, int64_t rows, Drop* out);
 int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D);
 int64_t stream_norm_bwd_scratch_bytes(int64_t B, int64_t S, int64_t D);
-int reduce_partials_impl(const float* part, int64_t B, int64_t slots, int W, float* out, cudaStream_t st, const char* what);
 int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, int wdtype, void* bi, void* y,
                          float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st);
 

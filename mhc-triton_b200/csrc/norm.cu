@@ -35,6 +35,7 @@ struct NormFwd {
   int group;             // columns per scale (GroupScale)
   int e8m0;
   float eps;
+  float inv_D;
   Drop drop;
 };
 
@@ -55,6 +56,7 @@ struct NormBwd {
   int parts;             // rows of dw_part
   int64_t chunks;        // per batch element (Mix)
   int tpc;               // tokens per chunk (Mix)
+  float inv_D;
   Drop drop;
 };
 
@@ -77,28 +79,29 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
 }
 
 // Scale of values whose largest magnitude is `amax`, and its reciprocal.  e8m0: the next power of two that is not
-// below amax / 448 (so nothing saturates), as its biased exponent; NaN and infinity become the NaN code 255.
-struct Scale { float inv; float f32; uint8_t code; };
+// below amax / 448 (so nothing saturates), as its biased exponent: 448 = 1.75 * 2^8, so that is amax's exponent - 8, plus
+// one if its mantissa is above 1.75, which the carry of an integer addition says exactly; NaN and infinity become the
+// NaN code 255.  No division: a scale per 32 columns made IEEE divisions a tenth of the kernel.
+struct Scale { float inv; float f32; uint32_t code; };
 __device__ __forceinline__ Scale make_scale(float amax, int e8m0) {
-  float s = __fdiv_rn(amax, kE4m3Max);
-  s = s < kMinScale ? kMinScale : s;  // false for NaN
   Scale r;
-  if (!e8m0) {
-    r.f32 = s;
-    r.inv = __fdiv_rn(1.f, s);
+  if (e8m0) {
+    const uint32_t b = __float_as_uint(amax);
+    const int e = (int)((b + 0x1fffffu) >> 23) - 8;
+    const bool finite = b < 0x7f800000u;
+    r.code = finite ? (uint32_t)(e < 1 ? 1 : e) : 255u;
+    r.f32 = 0.f;   // not stored
+    r.inv = finite ? __uint_as_float((254u - r.code) << 23) : __int_as_float(0x7fc00000);
+  } else {
+    const float s = amax * (1.f / kE4m3Max);
+    r.f32 = s < kMinScale ? kMinScale : s;  // false for NaN
+    r.inv = rcp_fast(r.f32);
     r.code = 0;
-    return r;
   }
-  const uint32_t b = __float_as_uint(s);
-  uint32_t e = (b >> 23) + ((b & 0x7fffffu) ? 1u : 0u);
-  if (!(s < __int_as_float(0x7f800000))) e = 255;
-  r.code = (uint8_t)e;
-  r.f32 = e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float(e << 23);
-  r.inv = e == 255 ? __int_as_float(0x7fc00000) : __uint_as_float((254u - e) << 23);
   return r;
 }
 __device__ __forceinline__ void store_scale(void* scales, int64_t i, const Scale& s, int e8m0) {
-  if (e8m0) ((uint8_t*)scales)[i] = s.code;
+  if (e8m0) ((uint8_t*)scales)[i] = (uint8_t)s.code;
   else ((float*)scales)[i] = s.f32;
 }
 
@@ -128,7 +131,7 @@ __device__ __forceinline__ void block_sum_max(float& sum, float& mx, float* sm) 
 // ------------------------------------------------------------------------------------- any width, any alignment
 // s[row, d], read element by element.
 template <typename T, Src SRC, bool DROP>
-__device__ __forceinline__ float src_at(const NormFwd& a, const DropKey& key, const float (&pre)[4], int64_t row, int64_t d) {
+__device__ __forceinline__ float src_at(const NormFwd& a, const DropSeed& seed, const float (&pre)[4], int64_t row, int64_t d) {
   if constexpr (SRC == Src::Mix) {
     const T* h = (const T*)a.x + row * 4 * a.D + d;
     const float b = ((pre[0] * to_f32(__ldg(h)) + pre[1] * to_f32(__ldg(h + a.D))) + pre[2] * to_f32(__ldg(h + 2 * a.D))) +
@@ -136,7 +139,7 @@ __device__ __forceinline__ float src_at(const NormFwd& a, const DropKey& key, co
     return a.sum_out ? to_f32(from_f32<T>(b)) : b;
   } else {
     float v[1] = {to_f32(__ldg((const T*)a.x + row * a.D + d))};
-    if constexpr (DROP) drop_apply<1>(a.drop, drop_bits<1>(a.drop, key, row, d), v);
+    if constexpr (DROP) drop_apply<1>(a.drop, drop_bits<1>(seed, drop_col(seed, (uint32_t)(d >> 3)), drop_row(a.drop, seed, row), d), v);
     if (a.res) v[0] += to_f32(__ldg((const T*)a.res + row * a.D + d));
     return v[0];
   }
@@ -154,27 +157,27 @@ k_norm_any_fwd(NormFwd a) {
 #pragma unroll
     for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + row / a.S * 4 + n);
   }
-  DropKey key{};
-  if constexpr (DROP) key = drop_key(a.drop);
+  DropSeed seed{};
+  if constexpr (DROP) seed = drop_seed(a.drop);
   float ss = 0.f, mx = 0.f;
   for (int64_t d = threadIdx.x; d < D; d += 256) {
-    const float v = src_at<T, SRC, DROP>(a, key, pre, row, d);
+    const float v = src_at<T, SRC, DROP>(a, seed, pre, row, d);
     if (a.sum_out) ((T*)a.sum_out)[row * D + d] = from_f32<T>(v);
     ss = fmaf(v, v, ss);
     if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v * load_w<T>(a.weight, a.w_f32, d)));
   }
   block_sum_max<OUT == Out::RowScale>(ss, mx, sm);
-  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + a.eps));
+  const float rstd = rsqrtf(ss * a.inv_D + a.eps);
   if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   if constexpr (OUT == Out::Plain) {
     for (int64_t d = threadIdx.x; d < D; d += 256)
       ((T*)a.y)[row * D + d] =
-          from_f32<T>(src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d));
+          from_f32<T>(src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d));
   } else if constexpr (OUT == Out::RowScale) {
     const Scale s = make_scale(mx * rstd, a.e8m0);
     if (threadIdx.x == 0) store_scale(a.scales, row, s, a.e8m0);
     for (int64_t d = threadIdx.x; d < D; d += 256) {
-      const float y = src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
+      const float y = src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
       ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y * s.inv, 0.f);
     }
   } else {  // a warp per group
@@ -187,7 +190,7 @@ k_norm_any_fwd(NormFwd a) {
         const int64_t d = g * a.group + j * 32 + lane;
         y[j] = 0.f;
         if (j * 32 < a.group && d < D)
-          y[j] = src_at<T, SRC, DROP>(a, key, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
+          y[j] = src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
         m = max_nan(m, fabsf(y[j]));
       }
 #pragma unroll
@@ -212,8 +215,8 @@ k_norm_any_bwd(NormBwd a) {
   __shared__ float sm[64];
   __shared__ float red[8 * 4];
   const int64_t D = a.D;
-  DropKey key{};
-  if constexpr (DROP) key = drop_key(a.drop);
+  DropSeed seed{};
+  if constexpr (DROP) seed = drop_seed(a.drop);
   float* dw = a.dw_part ? a.dw_part + (int64_t)blockIdx.x * D : nullptr;
   if (dw)
     for (int64_t d = threadIdx.x; d < D; d += 256) dw[d] = 0.f;
@@ -231,7 +234,7 @@ k_norm_any_bwd(NormBwd a) {
       const float rstd = __ldg(a.rstd + row);
       NormFwd f;
       f.x = a.x; f.res = a.res; f.sum_out = nullptr; f.D = D; f.drop = a.drop;
-      auto s_at = [&](int64_t d) -> float { return src_at<T, SRC, DROP>(f, key, pre, row, d); };
+      auto s_at = [&](int64_t d) -> float { return src_at<T, SRC, DROP>(f, seed, pre, row, d); };
       float c = 0.f, unused = 0.f;
       for (int64_t d = threadIdx.x; d < D; d += 256) {
         const float dy = to_f32(__ldg((const T*)a.dy + row * D + d)), s = s_at(d);
@@ -240,7 +243,7 @@ k_norm_any_bwd(NormBwd a) {
       }
       __syncthreads();  // the previous row's readers of sm are done
       block_sum_max<false>(c, unused, sm);
-      const float k = c * rstd * rstd * rstd / (float)D;
+      const float k = c * rstd * rstd * rstd * a.inv_D;
       for (int64_t d = threadIdx.x; d < D; d += 256) {
         const float dy = to_f32(__ldg((const T*)a.dy + row * D + d));
         float g[1] = {rstd * (dy * load_w<T>(a.weight, a.w_f32, d)) - s_at(d) * k};
@@ -256,7 +259,7 @@ k_norm_any_bwd(NormBwd a) {
           if (a.dsum) g[0] += to_f32(__ldg((const T*)a.dsum + row * D + d));
           if constexpr (DROP) {
             if (a.dres) ((T*)a.dres)[row * D + d] = from_f32<T>(g[0]);
-            drop_apply<1>(a.drop, drop_bits<1>(a.drop, key, row, d), g);
+            drop_apply<1>(a.drop, drop_bits<1>(seed, drop_col(seed, (uint32_t)(d >> 3)), drop_row(a.drop, seed, row), d), g);
           }
           ((T*)a.dx)[row * D + d] = from_f32<T>(g[0]);
         }
@@ -279,7 +282,7 @@ struct RowMap {
   int DV;    // packs per row
 };
 
-// Row sum (and NaN-keeping maximum) over the warps of one row; sm holds 2 x 16 floats.  One barrier.
+// Row sum (and NaN-keeping maximum) over the warps of one row (16 at most); sm holds 2 x 16 floats.  One barrier.
 template <bool MAX>
 __device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, const RowMap& m, int sub) {
 #pragma unroll
@@ -288,19 +291,19 @@ __device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, co
     if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (m.tpr == 32) return;
-  const int warp = threadIdx.x >> 5, nw = m.tpr >> 5;
+  const int warp = threadIdx.x >> 5, nw = m.tpr >> 5, l = threadIdx.x & 15;
   if ((threadIdx.x & 31) == 0) {
     sm[warp] = sum;
     if (MAX) sm[16 + warp] = mx;
   }
   __syncthreads();
-  float t = 0.f, x = 0.f;
-  for (int w = sub * nw; w < (sub + 1) * nw; ++w) {
-    t += sm[w];
-    if (MAX) x = max_nan(x, sm[16 + w]);
+  sum = l < nw ? sm[sub * nw + l] : 0.f;
+  if (MAX) mx = l < nw ? sm[16 + sub * nw + l] : 0.f;
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) {
+    sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
-  sum = t;
-  mx = x;
 }
 
 template <typename T, int V>
@@ -339,63 +342,69 @@ k_norm_fwd(NormFwd a, RowMap m) {
   __shared__ float sm[32];
   const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
   const int64_t row = (int64_t)blockIdx.x * m.rpc + sub, D = a.D;
-  const bool live = row < a.rows;
+  const int DV = row < a.rows ? m.DV : 0, stride = m.tpr * V;   // a row past the end owns no packs
   constexpr int NS = SRC == Src::Mix ? 4 : 2;
+  const T* xp = (const T*)a.x + (SRC == Src::Mix ? 4 : 1) * row * D + t * V;
+  const T* rp = (const T*)a.res + row * D + t * V;
   RawPack<T, V> raw[NP][NS];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int p = t + k * m.tpr;
 #pragma unroll
     for (int n = 0; n < NS; ++n) raw[k][n].w = make_uint4(0, 0, 0, 0);
-    if (live && p < m.DV) {
+    if (t + k * m.tpr < DV) {
       if constexpr (SRC == Src::Mix) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) raw[k][n] = ld_raw<T, V>((const T*)a.x + (row * 4 + n) * D + p * V);
+        for (int n = 0; n < 4; ++n) raw[k][n] = ld_raw<T, V>(xp + n * D + k * stride);
       } else {
-        raw[k][0] = ld_raw<T, V>((const T*)a.x + row * D + p * V);
-        if (a.res) raw[k][1] = ld_raw<T, V>((const T*)a.res + row * D + p * V);
+        raw[k][0] = ld_raw<T, V>(xp + k * stride);
+        if (a.res) raw[k][1] = ld_raw<T, V>(rp + k * stride);
       }
     }
   }
   float pre[4] = {0.f, 0.f, 0.f, 0.f};
   if constexpr (SRC == Src::Mix) {
-    if (live) {
+    if (DV) {
+      const float* h = a.hpre + (uint32_t)row / (uint32_t)a.S * 4;   // at most 2^31 rows
 #pragma unroll
-      for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + row / a.S * 4 + n);
+      for (int n = 0; n < 4; ++n) pre[n] = __ldg(h + n);
     }
   }
   float w[NP][V];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int p = t + k * m.tpr;
-    if (p < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, p * V, w[k]);
-    else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) w[k][e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) w[k][e] = 0.f;
+    if (t + k * m.tpr < DV) load_w_pack<T, V>(a.weight, a.w_f32, t * V + k * stride, w[k]);
   }
-  DropKey key{};
-  if constexpr (DROP) key = drop_key(a.drop);
+  DropSeed seed{};
+  DropRow drow{};
+  if constexpr (DROP) {
+    seed = drop_seed(a.drop);
+    drow = drop_row(a.drop, seed, row);
+  }
+  T* so = (T*)a.sum_out + row * D + t * V;
   float v[NP][V], ss = 0.f, mx = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int p = t + k * m.tpr;
-    const bool ok = live && p < m.DV;
+    const bool ok = t + k * m.tpr < DV;
     if constexpr (SRC == Src::Mix) {
 #pragma unroll
       for (int e = 0; e < V; ++e)
         v[k][e] = ((pre[0] * raw_get<V>(raw[k][0], e) + pre[1] * raw_get<V>(raw[k][1], e)) + pre[2] * raw_get<V>(raw[k][2], e)) +
                   pre[3] * raw_get<V>(raw[k][3], e);
-      if (a.sum_out && ok) PackIO<T, V>::store_round((T*)a.sum_out + row * D + p * V, v[k]);
+      if (a.sum_out && ok) PackIO<T, V>::store_round(so + k * stride, v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] = raw_get<V>(raw[k][0], e);
       if constexpr (DROP) {
-        if (ok) drop_apply<V>(a.drop, drop_bits<V>(a.drop, key, row, p * V), v[k]);
+        const int col = t * V + k * stride;
+        drop_apply<V>(a.drop, drop_bits<V>(seed, drop_col(seed, (uint32_t)col >> 3), drow, col), v[k]);
       }
+      if (a.res) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(raw[k][1], e);
-      if (a.sum_out && ok) PackIO<T, V>::store((T*)a.sum_out + row * D + p * V, v[k]);
+        for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(raw[k][1], e);
+      }
+      if (a.sum_out && ok) PackIO<T, V>::store(so + k * stride, v[k]);
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) {
@@ -404,64 +413,68 @@ k_norm_fwd(NormFwd a, RowMap m) {
     }
   }
   row_sum_max<OUT == Out::RowScale>(ss, mx, sm, m, sub);
-  const float rstd = __fdiv_rn(1.f, __fsqrt_rn(__fdiv_rn(ss, (float)D) + a.eps));
-  if (a.rstd && live && t == 0) a.rstd[row] = rstd;
+  const float rstd = rsqrtf(ss * a.inv_D + a.eps);
+  if (a.rstd && DV && t == 0) a.rstd[row] = rstd;
   Scale sc{};
   if constexpr (OUT == Out::RowScale) {
     sc = make_scale(mx * rstd, a.e8m0);
-    if (live && t == 0) store_scale(a.scales, row, sc, a.e8m0);
+    if (DV && t == 0) store_scale(a.scales, row, sc, a.e8m0);
   }
+  const int lanes = OUT == Out::GroupScale ? a.group / V : 1;          // group / V consecutive packs = consecutive lanes
+  const int64_t G = OUT == Out::GroupScale ? ((int)D + a.group - 1) / a.group : 1;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     const int p = t + k * m.tpr;
-    const bool ok = live && p < m.DV;
 #pragma unroll
     for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * rstd * w[k][e];
-    if constexpr (OUT == Out::GroupScale) {   // group / V consecutive packs = consecutive lanes
+    if constexpr (OUT == Out::GroupScale) {
       float g = 0.f;
 #pragma unroll
       for (int e = 0; e < V; ++e) g = max_nan(g, fabsf(v[k][e]));
-      const int lanes = a.group / V;
       for (int o = lanes >> 1; o > 0; o >>= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
       sc = make_scale(g, a.e8m0);
-      if (ok && (p & (lanes - 1)) == 0) store_scale(a.scales, row * ((D + a.group - 1) / a.group) + p / lanes, sc, a.e8m0);
+      if (p < DV && (p & (lanes - 1)) == 0) store_scale(a.scales, row * G + p / lanes, sc, a.e8m0);
     }
-    if (ok) {
-      if constexpr (OUT == Out::Plain) PackIO<T, V>::store((T*)a.y + row * D + p * V, v[k]);
-      else store_e4m3<V>((uint8_t*)a.y + row * D + p * V, v[k], sc.inv);
+    if (p < DV) {
+      if constexpr (OUT == Out::Plain) PackIO<T, V>::store((T*)a.y + row * D + t * V + k * stride, v[k]);
+      else store_e4m3<V>((uint8_t*)a.y + row * D + t * V + k * stride, v[k], sc.inv);
     }
   }
 }
 
 // Backward: persistent CTAs, so that the threads, which own the same columns in every row, keep the weight and
-// dweight's running sums in registers.  While a row is worked on the next one's packs are already on the way (PIPE).
-// An item is a row of rpc (Add) or a chunk of a batch element's tokens (Mix), walked rpc abreast.
-template <typename T, int V, int NP, Src SRC, bool DROP, bool PIPE>
+// dweight's running sums in registers.  The packs of the next DEPTH - 1 rows are on the way meanwhile, by cp.async into
+// slots of shared memory that only the thread itself reads (no barrier): in registers they spilled, and the
+// stream form ran at 42 % of the memory's rate.  An item is rpc rows (Add) or a chunk of a batch element's tokens
+// (Mix), walked rpc abreast.
+template <typename T, int V, int NP, int DEPTH, Src SRC, bool DROP>
 __global__ void __launch_bounds__(512)
 k_norm_bwd(NormBwd a, RowMap m) {
-  pdl_prologue();
+  extern __shared__ __align__(16) uint4 ring[];   // [DEPTH][NP][NS][threads]
   __shared__ float sm[2][32];
   __shared__ float red[16 * 4];
+  pdl_prologue();
   constexpr int NS = SRC == Src::Mix ? 5 : 4;   // Mix: dy, H[0..3]; Add: dy, x, residual, dsum
-  struct RowRaw {
-    RawPack<T, V> p[NP][NS];
-    float rstd;
-  };
   const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
   const int64_t D = a.D;
-  DropKey key{};
-  if constexpr (DROP) key = drop_key(a.drop);
+  const int stride = m.tpr * V;
+  const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16u, pitch = blockDim.x * 16u;
+  DropSeed seed{};
+  DropCol dcol[DROP ? NP : 1];
+  if constexpr (DROP) {
+    seed = drop_seed(a.drop);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) dcol[k] = drop_col(seed, (uint32_t)(t * V + k * stride) >> 3);
+  }
   float w[NP][V], dw[NP][V];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const int p = t + k * m.tpr;
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[k][e] = w[k][e] = 0.f;
-    if (p < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, p * V, w[k]);
+    if (t + k * m.tpr < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, t * V + k * stride, w[k]);
   }
-  const float inv_D = __fdiv_rn(1.f, (float)D);
 
-  // where this CTA is: rows base .. base + rpc - 1 of the item, the item's end, the item
+  // where the CTA is: rows base .. base + rpc - 1 of the item, the item's end
   struct Pos { int64_t item, base, end; };
   auto enter = [&](Pos& q) {   // first rows of q.item
     if (q.item >= a.items) return;
@@ -482,34 +495,74 @@ k_norm_bwd(NormBwd a, RowMap m) {
     }
     return q;
   };
-  auto load = [&](RowRaw& r, const Pos& q) {
+  auto issue = [&](int stage, const Pos& q) -> float {   // starts the copies of a row; its rstd
     const int64_t row = q.base + sub;
-    const bool live = q.item < a.items && row < q.end;
-    r.rstd = live ? __ldg(a.rstd + row) : 0.f;
+    float rstd = 0.f;
+    if (q.item < a.items && row < q.end) {
+      rstd = __ldg(a.rstd + row);
+      const T* src[NS];
+      src[0] = (const T*)a.dy + row * D + t * V;
+      if constexpr (SRC == Src::Mix) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      const int p = t + k * m.tpr;
-#pragma unroll
-      for (int n = 0; n < NS; ++n) r.p[k][n].w = make_uint4(0, 0, 0, 0);
-      if (live && p < m.DV) {
-        r.p[k][0] = ld_raw<T, V>((const T*)a.dy + row * D + p * V);
-        if constexpr (SRC == Src::Mix) {
-#pragma unroll
-          for (int n = 0; n < 4; ++n) r.p[k][1 + n] = ld_raw<T, V>((const T*)a.x + (row * 4 + n) * D + p * V);
-        } else {
-          r.p[k][1] = ld_raw<T, V>((const T*)a.x + row * D + p * V);
-          if (a.res) r.p[k][2] = ld_raw<T, V>((const T*)a.res + row * D + p * V);
-          if (a.dsum) r.p[k][3] = ld_raw<T, V>((const T*)a.dsum + row * D + p * V);
-        }
+        for (int n = 0; n < 4; ++n) src[1 + n] = (const T*)a.x + (row * 4 + n) * D + t * V;
+      } else {
+        src[1] = (const T*)a.x + row * D + t * V;
+        src[2] = (const T*)a.res + row * D + t * V;
+        src[3] = (const T*)a.dsum + row * D + t * V;
       }
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        if (t + k * m.tpr < m.DV) {
+#pragma unroll
+          for (int n = 0; n < NS; ++n)
+            if (SRC == Src::Mix || n < 2 || (n == 2 ? a.res : a.dsum))
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mine + (uint32_t)((stage * NP + k) * NS + n) * pitch),
+                           "l"(src[n] + k * stride)
+                           : "memory");
+        }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    return rstd;
   };
+  auto slot = [&](int stage, int k, int n) -> RawPack<T, V> {
+    RawPack<T, V> r;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.w.x), "=r"(r.w.y), "=r"(r.w.z), "=r"(r.w.w)
+                 : "r"(mine + (uint32_t)((stage * NP + k) * NS + n) * pitch)
+                 : "memory");
+    return r;
+  };
+
   float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
   int64_t pre_of = -1;
-  int parity = 0;
-  auto work = [&](const RowRaw& r, const Pos& q, bool last_of_item) {
+  int parity = 0, stage = 0;
+  float ahead[DEPTH > 1 ? DEPTH - 1 : 1];   // rstd of the rows on the way
+  Pos q{(int64_t)blockIdx.x, 0, 0};
+  enter(q);
+  Pos qi = q;
+#pragma unroll
+  for (int d = 0; d < DEPTH - 1; ++d) {
+    ahead[d] = issue(d, qi);
+    qi = next(qi);
+  }
+  while (q.item < a.items) {
+    float rstd;
+    if constexpr (DEPTH == 1) {
+      rstd = issue(0, q);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else {
+      rstd = ahead[0];
+#pragma unroll
+      for (int d = 0; d + 1 < DEPTH - 1; ++d) ahead[d] = ahead[d + 1];
+      ahead[DEPTH - 2] = issue(stage == 0 ? DEPTH - 1 : stage - 1, qi);   // the stage read in the previous iteration
+      qi = next(qi);
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    }
     const int64_t row = q.base + sub;
-    const bool live = row < q.end;
+    const int DV = row < q.end ? m.DV : 0;
+    const Pos q2 = next(q);
+    DropRow drow{};
+    if constexpr (DROP) drow = drop_row(a.drop, seed, row);
     if constexpr (SRC == Src::Mix) {
       if (q.item != pre_of) {
         pre_of = q.item;
@@ -517,129 +570,145 @@ k_norm_bwd(NormBwd a, RowMap m) {
         for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + q.item / a.chunks * 4 + n);
       }
     }
-    float s[NP][V], c = 0.f, unused = 0.f;
+    float s[NP][V], h[NP][V], c = 0.f, unused = 0.f;
     DropBits<V> bits[DROP ? NP : 1];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int p = t + k * m.tpr;
-      if constexpr (SRC == Src::Mix) {
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          s[k][e] = ((pre[0] * raw_get<V>(r.p[k][1], e) + pre[1] * raw_get<V>(r.p[k][2], e)) +
-                     pre[2] * raw_get<V>(r.p[k][3], e)) + pre[3] * raw_get<V>(r.p[k][4], e);
-      } else {
+      for (int e = 0; e < V; ++e) s[k][e] = h[k][e] = 0.f;
+      if (t + k * m.tpr < DV) {
+        const RawPack<T, V> dy = slot(stage, k, 0);
+        if constexpr (SRC == Src::Mix) {
+          RawPack<T, V> x[4];
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(r.p[k][1], e);
-        if constexpr (DROP) {
-          bits[k] = drop_bits<V>(a.drop, key, row, p * V);
-          drop_apply<V>(a.drop, bits[k], s[k]);
+          for (int n = 0; n < 4; ++n) x[n] = slot(stage, k, 1 + n);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            s[k][e] = ((pre[0] * raw_get<V>(x[0], e) + pre[1] * raw_get<V>(x[1], e)) + pre[2] * raw_get<V>(x[2], e)) +
+                      pre[3] * raw_get<V>(x[3], e);
+        } else {
+          const RawPack<T, V> x = slot(stage, k, 1);
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(x, e);
+          if constexpr (DROP) {
+            bits[k] = drop_bits<V>(seed, dcol[k], drow, t * V + k * stride);
+            drop_apply<V>(a.drop, bits[k], s[k]);
+          }
+          if (a.res) {
+            const RawPack<T, V> r = slot(stage, k, 2);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r, e);
+          }
         }
 #pragma unroll
-        for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r.p[k][2], e);
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float dy = raw_get<V>(r.p[k][0], e);
-        c = fmaf(dy * w[k][e], s[k][e], c);
-        dw[k][e] = fmaf(dy, s[k][e] * r.rstd, dw[k][e]);
+        for (int e = 0; e < V; ++e) {
+          const float g = raw_get<V>(dy, e);
+          h[k][e] = g * w[k][e];
+          c = fmaf(h[k][e], s[k][e], c);
+          dw[k][e] = fmaf(g, s[k][e] * rstd, dw[k][e]);
+        }
       }
     }
     row_sum_max<false>(c, unused, sm[parity], m, sub);
     parity ^= 1;   // the next row's sums go to the other half: nobody can still be reading it
-    const float kk = c * r.rstd * r.rstd * r.rstd * inv_D;
+    const float kk = c * rstd * rstd * rstd * a.inv_D;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int p = t + k * m.tpr;
-      const bool ok = live && p < m.DV;
-      float g[V];
+      if (t + k * m.tpr < DV) {
+        float g[V];
 #pragma unroll
-      for (int e = 0; e < V; ++e) g[e] = r.rstd * (raw_get<V>(r.p[k][0], e) * w[k][e]) - s[k][e] * kk;
-      if constexpr (SRC == Src::Mix) {
+        for (int e = 0; e < V; ++e) g[e] = rstd * h[k][e] - s[k][e] * kk;
+        if constexpr (SRC == Src::Mix) {
+          T* o = (T*)a.dx + row * 4 * D + t * V + k * stride;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          float o[V];
+          for (int n = 0; n < 4; ++n) {
+            const RawPack<T, V> x = slot(stage, k, 1 + n);
+            float u[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            acc[n] = fmaf(g[e], raw_get<V>(r.p[k][1 + n], e), acc[n]);
-            o[e] = pre[n] * g[e];
+            for (int e = 0; e < V; ++e) {
+              acc[n] = fmaf(g[e], raw_get<V>(x, e), acc[n]);
+              u[e] = pre[n] * g[e];
+            }
+            PackIO<T, V>::store(o + n * D, u);
           }
-          if (ok) PackIO<T, V>::store((T*)a.dx + (row * 4 + n) * D + p * V, o);
-        }
-      } else {
+        } else {
+          if (a.dsum) {
+            const RawPack<T, V> ds = slot(stage, k, 3);
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[e] += raw_get<V>(r.p[k][3], e);
-        if constexpr (DROP) {
-          if (ok && a.dres) PackIO<T, V>::store((T*)a.dres + row * D + p * V, g);
-          drop_apply<V>(a.drop, bits[k], g);
+            for (int e = 0; e < V; ++e) g[e] += raw_get<V>(ds, e);
+          }
+          if constexpr (DROP) {
+            if (a.dres) PackIO<T, V>::store((T*)a.dres + row * D + t * V + k * stride, g);
+            drop_apply<V>(a.drop, bits[k], g);
+          }
+          PackIO<T, V>::store((T*)a.dx + row * D + t * V + k * stride, g);
         }
-        if (ok) PackIO<T, V>::store((T*)a.dx + row * D + p * V, g);
       }
     }
     if constexpr (SRC == Src::Mix) {
-      if (last_of_item) {
+      if (q2.item != q.item) {
         __syncthreads();   // the previous item's readers of red are done
         block_reduce_store<4>(acc, a.dpre_part + q.item * 4, red);
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[n] = 0.f;
       }
     }
-  };
-
-  Pos q{(int64_t)blockIdx.x, 0, 0};
-  enter(q);
-  if constexpr (PIPE) {
-    RowRaw ra, rb;
-    load(ra, q);
-    while (q.item < a.items) {
-      const Pos q2 = next(q);
-      load(rb, q2);
-      work(ra, q, q2.item != q.item);
-      if (q2.item >= a.items) break;
-      q = next(q2);
-      load(ra, q);
-      work(rb, q2, q.item != q2.item);
-    }
-  } else {
-    RowRaw ra;
-    while (q.item < a.items) {
-      load(ra, q);
-      const Pos q2 = next(q);
-      work(ra, q, q2.item != q.item);
-      q = q2;
-    }
+    q = q2;
+    stage = stage + 1 == DEPTH ? 0 : stage + 1;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (a.dw_part) {
-    float* o = a.dw_part + ((int64_t)blockIdx.x * m.rpc + sub) * D;
+    float* o = a.dw_part + ((int64_t)blockIdx.x * m.rpc + sub) * D + t * V;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      const int p = t + k * m.tpr;
-      if (p < m.DV) {
+      if (t + k * m.tpr < m.DV) {
 #pragma unroll
         for (int e = 0; e < V; e += 4)
-          *reinterpret_cast<float4*>(o + p * V + e) = make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]);
+          *reinterpret_cast<float4*>(o + k * stride + e) = make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]);
       }
     }
   }
 }
 
-// out[d] = sum_i part[i, d] in fp64, fixed order: eight threads per column take rows i, i + 8, ..., joined in order.
+// Ends the backward, both sums in fp64 and a fixed order.  CTAs [0, wide): out[d] = sum_i part[i, d], 32 columns per CTA, 32
+// threads per column that take rows i, i + 32, ...  CTA wide + b: dH_pre[b] from its chunks' four sums.
 template <typename T>
-__global__ void __launch_bounds__(256)
-k_norm_dweight(const float* __restrict__ part, int64_t n, int64_t D, T* __restrict__ out) {
+__global__ void __launch_bounds__(1024)
+k_norm_finish(const float* __restrict__ part, int n, int64_t D, T* __restrict__ out, int wide,
+              const float* __restrict__ pre_part, int64_t chunks, float* __restrict__ dpre) {
   pdl_prologue();
-  __shared__ double sm[8][32];
+  __shared__ double sm[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t d = (int64_t)blockIdx.x * 32 + c;
-  double t = 0.0;
-  if (d < D)
-    for (int64_t i = g; i < n; i += 8) t += (double)__ldg(part + i * D + d);
-  sm[g][c] = t;
-  __syncthreads();
-  if (g == 0 && d < D) {
-    double s = 0.0;
+  double s = 0.0;
+  if ((int)blockIdx.x < wide) {
+    const int64_t d = (int64_t)blockIdx.x * 32 + c;
+    if (d < D) {
+      const float* p = part + (int64_t)g * D + d;
+      for (int i = g; i < n; i += 32 * 4, p += 32 * 4 * D) {   // four loads in flight
+        float v[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += sm[j][c];
-    out[d] = from_f32<T>((float)s);
+        for (int u = 0; u < 4; ++u) v[u] = i + 32 * u < n ? __ldg(p + (int64_t)32 * u * D) : 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s += (double)v[u];
+      }
+    }
+    sm[g][c] = s;
+    __syncthreads();
+    s = warp_sum_f64(sm[c][g]);            // warp g adds the 32 sums of column g
+    const int64_t col = (int64_t)blockIdx.x * 32 + g;
+    if (c == 0 && col < D) out[col] = from_f32<T>((float)s);
+  } else {
+    const int64_t b = (int64_t)blockIdx.x - wide;
+    const float* p = pre_part + b * chunks * 4;
+    for (int64_t i = threadIdx.x; i < chunks * 4; i += 1024) s += (double)__ldg(p + i);   // thread i: sum i % 4
+#pragma unroll
+    for (int o = 16; o >= 4; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    if (c < 4) sm[g][c] = s;
+    __syncthreads();
+    if (g < 4) {
+      s = warp_sum_f64(sm[c][g]);
+      if (c == 0) dpre[b * 4 + g] = (float)s;
+    }
   }
 }
 
@@ -659,6 +728,16 @@ static int64_t mix_tpc(int64_t S, int rpc) {
   return n > 0 ? n : 1;
 }
 static int64_t mix_chunks(int64_t S, int rpc) { return (S + mix_tpc(S, rpc) - 1) / mix_tpc(S, rpc); }
+
+// Shared memory of an SM that the resident CTAs' rings may use together (each has a few hundred bytes of its own beside).
+constexpr size_t kRingBytes = 220 * 1024;
+
+// launch_k for a kernel whose dynamic shared memory may exceed the 48 KiB it gets without asking .
+template <typename... KArgs, typename... Args>
+static void launch_ring(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {
+  if (smem > 48 * 1024) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  launch_k(kernel, grid, block, smem, st, std::forward<Args>(args)...);
+}
 
 // Threads and rows per CTA for rows of D elements in packs of V: `np` packs per thread.
 static RowMap row_map(int64_t D, int V, int np) {
@@ -745,19 +824,28 @@ static int launch_bwd(const char* what, NormBwd& a, float* scratch, int dtype, c
   scratch = (float*)(((uintptr_t)scratch + 15) & ~(uintptr_t)15);
   if (a.dw_part) { a.dw_part = scratch; scratch += a.parts * a.D; }
   a.dpre_part = scratch;
+  const int per_sm = threads > 256 ? 1 : 2;
+  const size_t stage = (size_t)threads * np * (SRC == Src::Mix ? 5 : 4) * 16;
   if (np == 0)
     MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_bwd<T, SRC, DROP>, (unsigned)ctas, 256, 0, st, a)));
-  else if (np == 2)
-    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, vec_width<T>::value, 2, SRC, DROP, true>, (unsigned)ctas, threads, 0, st, a, m)));
+  else if (np == 4)
+    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_bwd<T, vec_width<T>::value, 4, 1, SRC, DROP>, (unsigned)ctas, threads, stage, st, a, m)));
+  else if (3 * stage <= kRingBytes / per_sm)
+    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_bwd<T, vec_width<T>::value, 2, 3, SRC, DROP>, (unsigned)ctas, threads, 3 * stage, st, a, m)));
   else
-    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, vec_width<T>::value, 4, SRC, DROP, false>, (unsigned)ctas, threads, 0, st, a, m)));
+    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_bwd<T, vec_width<T>::value, 2, 2, SRC, DROP>, (unsigned)ctas, threads, 2 * stage, st, a, m)));
   return check_launch(what);
 }
 
-static int finish_dweight(const char* what, const float* part, int64_t ctas, int64_t D, void* dweight, int wdtype,
-                          cudaStream_t st) {
-  ProfScope ps("k_norm_dweight", st);
-  MHC_TYPE_DISPATCH(wdtype, (launch_k(k_norm_dweight<T>, (unsigned)((D + 31) / 32), 256, 0, st, part, ctas, D, (T*)dweight)));
+// dweight (null: none) from the CTAs' partial rows, dH_pre (Mix; null: none) from the chunks' sums.
+static int finish_bwd(const char* what, const NormBwd& a, void* dweight, int wdtype, float* dpre, int64_t B, cudaStream_t st) {
+  if (!dweight && !dpre) return MHC_OK;
+  const int wide = dweight ? (int)((a.D + 31) / 32) : 0;
+  const int64_t grid = wide + (dpre ? B : 0);
+  if (grid > kMaxGridItems) return fail(MHC_ERR_BAD_SHAPE, "%s: too many batch elements", what);
+  ProfScope ps("k_norm_finish", st);
+  MHC_TYPE_DISPATCH(wdtype, (launch_k(k_norm_finish<T>, (unsigned)grid, 1024, 0, st, (const float*)a.dw_part, a.parts, a.D,
+                                      (T*)dweight, wide, (const float*)a.dpre_part, a.chunks, dpre)));
   return check_launch(what);
 }
 
@@ -765,7 +853,7 @@ int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, 
                          float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st) {
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = wdtype == MHC_F32; a.sum_out = bi; a.y = y; a.rstd = rstd;
-  a.rows = B * S; a.S = S; a.D = D; a.eps = eps;
+  a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
   return launch_fwd<Src::Mix, false, Out::Plain>("stream_norm_fwd", a, dtype, st);
 }
 
@@ -786,7 +874,7 @@ extern "C" int mhc_add_rms_norm_fwd(const void* x, const void* residual, const v
   if (rows == 0 || D == 0) return MHC_OK;
   if (!x || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = y;
-  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps;
+  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
   cudaStream_t st = (cudaStream_t)stream;
   return drop ? launch_fwd<Src::Add, true, Out::Plain>(what, a, dtype, st)
               : launch_fwd<Src::Add, false, Out::Plain>(what, a, dtype, st);
@@ -804,7 +892,7 @@ extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, c
   NormFwd a{};
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = q;
   a.scales = scales; a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0;
-  a.rows = rows; a.S = 1; a.D = D; a.eps = eps;
+  a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Add, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Add, false, Out::RowScale>(what, a, dtype, st);
@@ -835,11 +923,11 @@ extern "C" int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* x,
   if (!is_aligned_to(scratch, 4)) return fail(MHC_ERR_MISALIGNED, "%s: scratch must be 4-byte aligned", what);
   if (!drop && dresidual) return fail(MHC_ERR_BAD_ARGUMENT, "%s: without dropout the residual's gradient is dx", what);
   a.dy = dy; a.dsum = dsum; a.x = x; a.res = residual; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32;
-  a.dx = dx; a.dres = dresidual; a.dw_part = dweight ? (float*)scratch : nullptr; a.items = rows; a.D = D;
+  a.dx = dx; a.dres = dresidual; a.dw_part = dweight ? (float*)scratch : nullptr; a.items = rows; a.D = D; a.inv_D = (float)(1.0 / (double)D);
   if (int e = drop ? launch_bwd<Src::Add, true>(what, a, (float*)scratch, dtype, st)
                    : launch_bwd<Src::Add, false>(what, a, (float*)scratch, dtype, st))
     return e;
-  return dweight ? finish_dweight(what, a.dw_part, a.parts, D, dweight, weight_dtype, st) : MHC_OK;
+  return finish_bwd(what, a, dweight, weight_dtype, nullptr, 0, st);
 }
 
 extern "C" int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
@@ -867,7 +955,7 @@ extern "C" int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, cons
   if (!H || !H_pre || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q; a.scales = scales;
-  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps;
+  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Mix, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Mix, false, Out::RowScale>(what, a, dtype, st);
@@ -898,7 +986,7 @@ extern "C" int mhc_stream_norm_bwd(const void* dy, const void* H, const float* H
   NormBwd a{};
   a.dy = dy; a.x = H; a.hpre = H_pre; a.rstd = rstd; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.dx = dH;
   a.dw_part = dweight ? (float*)scratch : nullptr; a.items = B; a.S = S; a.D = D;
+  a.inv_D = (float)(1.0 / (double)D);
   if (int e = launch_bwd<Src::Mix, false>(what, a, (float*)scratch, dtype, st)) return e;
-  if (int e = reduce_partials_impl(a.dpre_part, B, a.chunks, 4, dH_pre, st, what)) return e;
-  return dweight ? finish_dweight(what, a.dw_part, a.parts, D, dweight, weight_dtype, st) : MHC_OK;
+  return finish_bwd(what, a, dweight, weight_dtype, dH_pre, B, st);
 }

@@ -22,25 +22,56 @@ struct Drop {
   uint32_t row0;       // added to the row index
 };
 
-struct DropKey { uint32_t k0, k1, c2, c3; };
+// The ten rounds, split by what they depend on.  With the counter (column / 8, row, offset) the multiplications of
+// rounds 1 to 3 depend on the column or on the row alone: a thread that stays in its columns and walks rows does the
+// column's part once (DropCol), the row's single multiplication once per row (DropRow), and 15 of the 20
+// multiplications per block.
+struct DropSeed { uint32_t k0, k1, row_x, c1, c3; };  // row_x, c1: what round 1 makes of the offset's low word
+struct DropCol { uint32_t x, y, z, c3; };
+struct DropRow { uint32_t hi, lo; };
 
-__device__ __forceinline__ DropKey drop_key(const Drop& d) {
+constexpr uint32_t kPhiloxM0 = 0xD2511F53u, kPhiloxM1 = 0xCD9E8D57u, kPhiloxW0 = 0x9E3779B9u, kPhiloxW1 = 0xBB67AE85u;
+
+__device__ __forceinline__ DropSeed drop_seed(const Drop& d) {
   const uint64_t seed = (uint64_t)__ldg((const unsigned long long*)d.rng);
   const uint64_t off = (uint64_t)__ldg((const unsigned long long*)d.rng + 1);
-  return DropKey{(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)off, (uint32_t)(off >> 32)};
+  const uint64_t b = (uint64_t)(uint32_t)off * kPhiloxM1;
+  DropSeed s;
+  s.k0 = (uint32_t)seed;
+  s.k1 = (uint32_t)(seed >> 32);
+  s.row_x = (uint32_t)(b >> 32) ^ s.k0;
+  s.c1 = (uint32_t)b;
+  s.c3 = (uint32_t)(off >> 32);
+  return s;
 }
 
-__device__ __forceinline__ uint4 philox4x32_10(const DropKey& key, uint32_t col8, uint32_t row) {
-  uint32_t c0 = col8, c1 = row, c2 = key.c2, c3 = key.c3, k0 = key.k0, k1 = key.k1;
+__device__ __forceinline__ DropCol drop_col(const DropSeed& s, uint32_t col8) {
+  const uint64_t a1 = (uint64_t)col8 * kPhiloxM0;                               // round 1
+  const uint64_t b2 = (uint64_t)((uint32_t)(a1 >> 32) ^ s.c3 ^ s.k1) * kPhiloxM1;  // round 2
+  const uint64_t a3 = (uint64_t)((uint32_t)(b2 >> 32) ^ s.c1 ^ (s.k0 + kPhiloxW0)) * kPhiloxM0;  // round 3
+  DropCol c;
+  c.x = (uint32_t)a1 ^ (s.k1 + kPhiloxW1);
+  c.y = (uint32_t)b2 ^ (s.k0 + 2 * kPhiloxW0);
+  c.z = (uint32_t)(a3 >> 32) ^ (s.k1 + 2 * kPhiloxW1);
+  c.c3 = (uint32_t)a3;
+  return c;
+}
+
+__device__ __forceinline__ DropRow drop_row(const Drop& d, const DropSeed& s, int64_t row) {
+  const uint64_t a2 = (uint64_t)(s.row_x ^ ((uint32_t)row + d.row0)) * kPhiloxM0;  // round 2
+  return DropRow{(uint32_t)(a2 >> 32), (uint32_t)a2};
+}
+
+__device__ __forceinline__ uint4 drop_block(const DropSeed& s, const DropCol& col, const DropRow& row) {
+  const uint64_t b3 = (uint64_t)(row.hi ^ col.x) * kPhiloxM1;                   // round 3
+  uint32_t c0 = (uint32_t)(b3 >> 32) ^ col.y, c1 = (uint32_t)b3, c2 = col.z ^ row.lo, c3 = col.c3;
 #pragma unroll
-  for (int i = 0; i < 10; ++i) {
-    const uint64_t a = (uint64_t)c0 * 0xD2511F53u, b = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(b >> 32) ^ c1 ^ k0;
+  for (int i = 3; i < 10; ++i) {
+    const uint64_t a = (uint64_t)c0 * kPhiloxM0, b = (uint64_t)c2 * kPhiloxM1;
+    c0 = (uint32_t)(b >> 32) ^ c1 ^ (s.k0 + (uint32_t)i * kPhiloxW0);
     c1 = (uint32_t)b;
-    c2 = (uint32_t)(a >> 32) ^ c3 ^ k1;
+    c2 = (uint32_t)(a >> 32) ^ c3 ^ (s.k1 + (uint32_t)i * kPhiloxW1);
     c3 = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
   return make_uint4(c0, c1, c2, c3);
 }
@@ -49,8 +80,8 @@ __device__ __forceinline__ uint4 philox4x32_10(const DropKey& key, uint32_t col8
 template <int V> struct DropBits { uint32_t w[V > 1 ? V / 2 : 1]; };
 
 template <int V>
-__device__ __forceinline__ DropBits<V> drop_bits(const Drop& d, const DropKey& key, int64_t row, int64_t col) {
-  const uint4 r = philox4x32_10(key, (uint32_t)(col >> 3), (uint32_t)row + d.row0);
+__device__ __forceinline__ DropBits<V> drop_bits(const DropSeed& s, const DropCol& dc, const DropRow& dr, int64_t col) {
+  const uint4 r = drop_block(s, dc, dr);
   DropBits<V> o;
   if constexpr (V == 1) {  // the half the column owns, in the upper half of the word
     const int e = (int)(col & 7);

@@ -188,12 +188,13 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
   pdl_prologue();
   const Item it = decode_item(g);
   if (it.col >= g.DV) return;
-  DropKey key{};
-  if constexpr (DROP) key = drop_key(drop);
   float p[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
   const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
+  DropSeed seed{};
+  DropCol dcol{};
+  if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
   using B5 = Bundle<T, V, 5>;
   for_tokens<MHC_ADDFWD_PIPE != 0, B5>(
       it.s0 + it.sub, it.s1, g.sub,
@@ -206,7 +207,7 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
       [&](const B5& u, int64_t s) {
         float y[V], x[V];
         unpack<T, V>(u.p[4], y);
-        if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
+        if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
         T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -249,8 +250,9 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
     for (int e = 0; e < V; ++e) acc[n][e] = 0.f;
   const bool live = it.col < g.DV;
   if (live) {
-    DropKey key{};
-    if constexpr (DROP) key = drop_key(drop);
+    DropSeed seed{};
+    DropCol dcol{};
+    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -264,7 +266,7 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
     auto compute = [&](const B5& u, int64_t s) {
       float y[V], x[V];
       unpack<T, V>(u.p[4], y);
-      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
+      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
       T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -358,8 +360,9 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
   const bool live = it.col < g.DV;
   if (!POOL && !live) return;
   if (live) {
-    DropKey key{};
-    if constexpr (DROP) key = drop_key(drop);
+    DropSeed seed{};
+    DropCol dcol{};
+    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
     float p[4], R[16];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -375,7 +378,7 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
     auto compute = [&](const B5& u, int64_t s) {
       float x[4][V], y[V], o[V];
       unpack<T, V>(u.p[4], y);
-      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(drop, key, tok + s, c0), y);
+      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
 #pragma unroll
       for (int n = 0; n < 4; ++n) unpack<T, V>(u.p[n], x[n]);
       T* op = Hn + (tok + s) * 4 * D + c0;
@@ -483,8 +486,9 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
     const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
-    DropKey key{};
-    if constexpr (DROP) key = drop_key(drop);
+    DropSeed seed{};
+    DropCol dcol{};
+    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
     using B5 = Bundle<T, V, 5>;
     for_tokens<MHC_ADDBWD_PIPE != 0, B5>(
         it.s0 + it.sub, it.s1, g.sub,
@@ -499,7 +503,7 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
           unpack<T, V>(u.p[4], y);
           DropBits<V> bits{};
           if constexpr (DROP) {
-            bits = drop_bits<V>(drop, key, tok + s, c0);
+            bits = drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0);
             drop_apply<V>(drop, bits, y);
           }
 #pragma unroll
@@ -948,10 +952,6 @@ static int launch_reduce(const float* part, int64_t B, int64_t slots, int W, int
     launch_k(k_reduce_partials, (unsigned)B, 256, 0, st, part, slots, W, W0, out0, out1);
   }
   return check_launch(what);
-}
-
-int reduce_partials_impl(const float* part, int64_t B, int64_t slots, int W, float* out, cudaStream_t st, const char* what) {
-  return launch_reduce(part, B, slots, W, W, out, nullptr, st, what);
 }
 
 }  // namespace mhc
