@@ -9,6 +9,9 @@ namespace mhc {
 // A thread owns one group of columns (a 16-byte pack; for V = 1, rows that do not divide into packs, 8 columns read one
 // by one) and walks kDropRows rows: the column's part of the generator is computed once and all loads are
 // issued before the first use.
+#ifndef MHC_DROPOUT_MINB
+#define MHC_DROPOUT_MINB 6
+#endif
 #ifndef MHC_DROP_ROWS
 #define MHC_DROP_ROWS 4
 #endif
@@ -22,31 +25,34 @@ struct DropGeo {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, MHC_DROPOUT_MINB)
 k_counter_dropout(const T* __restrict__ x, T* __restrict__ y, DropGeo g, Drop drop) {
   pdl_prologue();
   const int64_t chunk = g.CG == 1 ? blockIdx.x : blockIdx.x / g.CG;
   const int cg = g.CG == 1 ? 0 : (int)(blockIdx.x - chunk * g.CG);
   const int s = threadIdx.x / g.cols, pos = cg * g.cols + threadIdx.x - s * g.cols;
+  const DropSeed seed = drop_seed(drop);   // whole warps
   if (pos >= g.groups) return;
   const int64_t row0 = chunk * (kDropRows * g.sub) + s, step = g.sub;
-  const DropSeed seed = drop_seed(drop);
   if constexpr (V > 1) {
-    const int64_t col = (int64_t)pos * V;
+    const uint32_t col = (uint32_t)pos * V;
+    const int64_t left = g.rows - row0, jump = step * g.D;
+    const int n = left <= 0 ? 0 : left > (kDropRows - 1) * step ? kDropRows : (int)((left + step - 1) / step);   // rows to do
+    const T* xp = x + row0 * g.D + col;
+    T* yp = y + row0 * g.D + col;
     RawPack<T, V> raw[kDropRows];
 #pragma unroll
     for (int r = 0; r < kDropRows; ++r)
-      if (row0 + r * step < g.rows) raw[r] = ld_raw<T, V>(x + (row0 + r * step) * g.D + col);
-    const DropCol dc = drop_col(seed, (uint32_t)(col >> 3));
+      if (r < n) raw[r] = ld_raw<T, V>(xp + r * jump);
+    const DropCol dc = drop_col(seed, col >> 3);
 #pragma unroll
     for (int r = 0; r < kDropRows; ++r) {
-      const int64_t row = row0 + r * step;
-      if (row < g.rows) {
+      if (r < n) {
         float v[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) v[e] = raw_get<V>(raw[r], e);
-        drop_apply<V>(drop, drop_bits<V>(seed, dc, drop_row(drop, seed, row), col), v);
-        PackIO<T, V>::store(y + row * g.D + col, v);
+        drop_apply<V>(drop, drop_bits<V>(seed, dc, drop_row(drop, seed, row0 + r * step), col), v);
+        PackIO<T, V>::store(yp + r * jump, v);
       }
     }
   } else {

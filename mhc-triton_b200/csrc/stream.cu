@@ -3,6 +3,7 @@
 // Each thread owns one 16-byte pack position along D and walks the tokens of its chunk, so the
 // 20 mixing coefficients of the batch element (and, in the apply pass, the pooled-state gradient
 // of its columns) stay in registers and every warp access is 512 contiguous bytes.
+#include <algorithm>
 #include <initializer_list>
 
 #include "common.cuh"
@@ -179,32 +180,48 @@ k_stream_premix_fwd(const T* __restrict__ H, const float* __restrict__ Hpre, T* 
 }
 
 // ------------------------------------------------------------------------------ add residual
+// The forms with dropout take 3 times as many instructions per pack; loads in registers then leave too few warps to cover
+// both the memory and the generator's chain of multiplications (397 / 329 us forward / backward at 8 x 4096 x 4096
+// bf16, 357 / 247 without dropout).  They keep MHC_DROP_STAGES tokens in the shared-memory ring instead and walk more
+// tokens per CTA: 349 / 263 us.
+#ifndef MHC_DROP_STAGES
+#define MHC_DROP_STAGES 3
+#endif
+#ifndef MHC_TPC_DROPFWD
+#define MHC_TPC_DROPFWD 4
+#endif
+#ifndef MHC_TPC_DROPBWD
+#define MHC_TPC_DROPBWD 16   // at most, see drop_bwd_tpc
+#endif
+#ifndef MHC_DROP_MINB
+#define MHC_DROP_MINB 2
+#endif
 // DROP (here and in the other add-residual kernels): the branch output passes through the counter-based dropout of
 // rng.cuh on its way in (row = b * S + s); the mask is recomputed wherever it is needed.
 template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(MHC_MAX_COLS, MHC_ADDFWD_MINB)
+__global__ void __launch_bounds__(MHC_MAX_COLS, DROP ? MHC_DROP_MINB : MHC_ADDFWD_MINB)
 k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const float* __restrict__ Hpost,
                    T* __restrict__ Hn, Geo g, Drop drop) {
   pdl_prologue();
+  extern __shared__ __align__(16) float sm[];   // DROP: the ring
   const Item it = decode_item(g);
+  DropSeed seed{};
+  DropCol dcol{};
+  if constexpr (DROP) seed = drop_seed(drop);   // whole warps
   if (it.col >= g.DV) return;
   float p[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
   const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
-  DropSeed seed{};
-  DropCol dcol{};
-  if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
+  if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
   using B5 = Bundle<T, V, 5>;
-  for_tokens<MHC_ADDFWD_PIPE != 0, B5>(
-      it.s0 + it.sub, it.s1, g.sub,
-      [&](B5& u, int64_t s) {
+  auto load = [&](B5& u, int64_t s) {
         const T* r = Hr + (tok + s) * 4 * D + c0;
         u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
         for (int n = 0; n < 4; ++n) u.p[n] = ld_raw<T, V>(r + n * D);
-      },
-      [&](const B5& u, int64_t s) {
+      };
+  auto compute = [&](const B5& u, int64_t s) {
         float y[V], x[V];
         unpack<T, V>(u.p[4], y);
         if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
@@ -216,7 +233,16 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
           for (int e = 0; e < V; ++e) x[e] = x[e] + p[n] * y[e];
           PackIO<T, V>::store(o + n * D, x);
         }
-      });
+      };
+  if constexpr (DROP && V > 1)
+    for_tokens_staged<T, V, 5, MHC_DROP_STAGES>(
+        it.s0 + it.sub, it.s1, g.sub, (uint32_t)__cvta_generic_to_shared(sm),
+        [&](int64_t s, int n) -> const T* {
+          return n == 4 ? bo + (tok + s) * D + c0 : Hr + ((tok + s) * 4 + n) * D + c0;
+        },
+        compute);
+  else
+    for_tokens<MHC_ADDFWD_PIPE != 0, B5>(it.s0 + it.sub, it.s1, g.sub, load, compute);
 }
 
 // Add residual that also leaves the token sums of its own output for the NEXT layer's mean-pool:
@@ -249,10 +275,11 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
 #pragma unroll
     for (int e = 0; e < V; ++e) acc[n][e] = 0.f;
   const bool live = it.col < g.DV;
+  DropSeed seed{};
+  if constexpr (DROP) seed = drop_seed(drop);   // whole warps
   if (live) {
-    DropSeed seed{};
     DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
+    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -358,11 +385,12 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
       for (int e = 0; e < V; ++e) acc[POOL ? n : 0][e] = 0.f;
   }
   const bool live = it.col < g.DV;
+  DropSeed seed{};
+  if constexpr (DROP) seed = drop_seed(drop);   // whole warps
   if (!POOL && !live) return;
   if (live) {
-    DropSeed seed{};
     DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
+    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
     float p[4], R[16];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -473,32 +501,32 @@ __device__ __forceinline__ void finish_partials(const float* __restrict__ part, 
 #define MHC_ADDBWD_PIPE 1
 #endif
 template <typename T, int V, bool DROP>
-__global__ void __launch_bounds__(MHC_MAX_COLS, MHC_ADDBWD_MINB)
+__global__ void __launch_bounds__(MHC_MAX_COLS, DROP ? MHC_DROP_MINB : MHC_ADDBWD_MINB)
 k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const float* __restrict__ Hpost,
                    T* __restrict__ dbo, float* __restrict__ part, Geo g, int* tickets, float* __restrict__ dH_post,
                    Drop drop) {
+  extern __shared__ __align__(16) float sm[];   // DROP: the ring
   pdl_prologue();
   __shared__ __align__(8) float red[32 * 20];
   const Item it = decode_item(g);
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  DropSeed seed{};
+  if constexpr (DROP) seed = drop_seed(drop);   // whole warps
   if (it.col < g.DV) {
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
     const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
-    DropSeed seed{};
     DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed = drop_seed(drop), (uint32_t)(c0 >> 3));
+    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
     using B5 = Bundle<T, V, 5>;
-    for_tokens<MHC_ADDBWD_PIPE != 0, B5>(
-        it.s0 + it.sub, it.s1, g.sub,
-        [&](B5& u, int64_t s) {
+    auto load = [&](B5& u, int64_t s) {
           const T* gp = G + (tok + s) * 4 * D + c0;
           u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
           for (int n = 0; n < 4; ++n) u.p[n] = ld_raw<T, V>(gp + n * D);
-        },
-        [&](const B5& u, int64_t s) {
+        };
+    auto compute = [&](const B5& u, int64_t s) {
           float y[V], z[V], x[V];
           unpack<T, V>(u.p[4], y);
           DropBits<V> bits{};
@@ -519,7 +547,16 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
           }
           if constexpr (DROP) drop_apply<V>(drop, bits, z);
           PackIO<T, V>::store(dbo + (tok + s) * D + c0, z);
-        });
+        };
+    if constexpr (DROP && V > 1)
+      for_tokens_staged<T, V, 5, MHC_DROP_STAGES>(
+          it.s0 + it.sub, it.s1, g.sub, (uint32_t)__cvta_generic_to_shared(sm),
+          [&](int64_t s, int n) -> const T* {
+            return n == 4 ? bo + (tok + s) * D + c0 : G + ((tok + s) * 4 + n) * D + c0;
+          },
+          compute);
+    else
+      for_tokens<MHC_ADDBWD_PIPE != 0, B5>(it.s0 + it.sub, it.s1, g.sub, load, compute);
   }
   block_reduce_store<4>(acc, part + (it.b * geo_slots_dev(g) + it.slot) * 4, red);
   if (!tickets) return;
@@ -1000,14 +1037,16 @@ static int add_residual_fwd_impl(const void* H_residual, const void* branch_outp
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H_residual || !branch_output || !H_post || !H_new) return fail(MHC_ERR_NULL_POINTER, "add_residual_fwd: null pointer");
   const int vec = pick_vec(dtype, D, {H_residual, branch_output, H_new});
-  Geo g = make_geo(S, D, vec, GeoKind::Stream, MHC_TPC_ADDFWD);
+  const bool staged = drop && vec > 1;
+  Geo g = make_geo(S, D, vec, GeoKind::Stream, staged ? MHC_TPC_DROPFWD : MHC_TPC_ADDFWD);
+  const size_t smem = staged ? (size_t)MHC_DROP_STAGES * 5 * 16 * geo_block(g) : 0;
   g.reverse = (MHC_REV_MASK >> 2) & 1;
   const int64_t items = B * geo_slots(g);
   if (int e = check_grid("add_residual_fwd", items)) return e;
   cudaStream_t st = (cudaStream_t)stream;
   {
     ProfScope ps("k_add_residual_fwd", st);
-    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_k(k_add_residual_fwd<T, V, DROP>, (unsigned)items, geo_block(g), 0, st,
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_pool_k(k_add_residual_fwd<T, V, DROP>, (unsigned)items, geo_block(g), smem, st,
                                  (const T*)H_residual, (const T*)branch_output, H_post, (T*)H_new, g,
                                  drop ? *drop : Drop{})));
   }
@@ -1114,6 +1153,14 @@ extern "C" int mhc_add_residual_pool_fwd(const void* H_residual, const void* bra
                                     stream);
 }
 
+// Tokens per thread of the backward with dropout: MHC_TPC_DROPBWD, fewer (4 at least) where one batch element would not
+// fill the device's CTAs.  A function of S, D and the device only, as every chunk length is.
+static int drop_bwd_tpc(int64_t S, int64_t D, int vec) {
+  const Geo g = make_geo(S, D, vec, GeoKind::Reduce, 4);
+  const int64_t even = S * g.CG / ((int64_t)g.sub * MHC_DROP_MINB * sm_count());
+  return (int)std::min<int64_t>(std::max<int64_t>(even, 4), MHC_TPC_DROPBWD);
+}
+
 static int add_residual_bwd_impl(const void* dH_new, const void* branch_output, const float* H_post, const Drop* drop,
                                  void* d_branch_output, float* dH_post, void* scratch, int64_t scratch_bytes,
                                  int32_t* tickets, int64_t B, int64_t S, int64_t D, int dtype, mhc_stream_t stream) {
@@ -1127,7 +1174,10 @@ static int add_residual_bwd_impl(const void* dH_new, const void* branch_output, 
   }
   // sizes first, pointers last: a call whose scratch is too small says so even with null pointers
   const int vec = pick_vec(dtype, D, {dH_new, branch_output, d_branch_output});
-  Geo g = make_geo(S, D, vec, GeoKind::Reduce, MHC_TPC_ADDBWD, MHC_ADDBWD_OCC, MHC_FIT_COLS != 0, MHC_NARROW_MULT);
+  const bool staged = drop && vec > 1;
+  Geo g = staged ? make_geo(S, D, vec, GeoKind::Reduce, drop_bwd_tpc(S, D, vec), MHC_DROP_MINB)
+                 : make_geo(S, D, vec, GeoKind::Reduce, MHC_TPC_ADDBWD, MHC_ADDBWD_OCC, MHC_FIT_COLS != 0, MHC_NARROW_MULT);
+  const size_t smem = staged ? (size_t)MHC_DROP_STAGES * 5 * 16 * geo_block(g) : 0;
   g.reverse = (MHC_REV_MASK >> 3) & 1;
   const int64_t slots = geo_slots(g), items = B * slots;
   if (int e = check_grid("add_residual_bwd", items)) return e;
@@ -1141,7 +1191,7 @@ static int add_residual_bwd_impl(const void* dH_new, const void* branch_output, 
   if (!ticket_finish_supported()) tickets = nullptr;
   {
     ProfScope ps("k_add_residual_bwd", st);
-    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_k(k_add_residual_bwd<T, V, DROP>, (unsigned)items, geo_block(g), 0, st,
+    MHC_DROP_DISPATCH(dtype, vec, drop, (launch_pool_k(k_add_residual_bwd<T, V, DROP>, (unsigned)items, geo_block(g), smem, st,
                                  (const T*)dH_new, (const T*)branch_output, H_post, (T*)d_branch_output,
                                  (float*)scratch, g, (int*)tickets, dH_post, drop ? *drop : Drop{})));
   }
