@@ -6,14 +6,13 @@
 
 namespace mhc {
 
-// A thread owns one group of columns (a 16-byte pack; for V = 1, rows that do not divide into packs, 8 columns read one
-// by one) and walks kDropRows rows: the column's part of the generator is computed once and all loads are
-// issued before the first use.
+// A thread owns one 16-byte pack of columns and walks kDropRows rows: the column's part of the generator is computed once
+// and all loads are issued before the first use.
 #ifndef MHC_DROPOUT_MINB
 #define MHC_DROPOUT_MINB 6
 #endif
 #ifndef MHC_DROP_ROWS
-#define MHC_DROP_ROWS 4
+#define MHC_DROP_ROWS 5
 #endif
 constexpr int kDropRows = MHC_DROP_ROWS;
 struct DropGeo {
@@ -34,43 +33,60 @@ k_counter_dropout(const T* __restrict__ x, T* __restrict__ y, DropGeo g, Drop dr
   const DropSeed seed = drop_seed(drop);   // whole warps
   if (pos >= g.groups) return;
   const int64_t row0 = chunk * (kDropRows * g.sub) + s, step = g.sub;
-  if constexpr (V > 1) {
-    const uint32_t col = (uint32_t)pos * V;
-    const int64_t left = g.rows - row0, jump = step * g.D;
-    const int n = left <= 0 ? 0 : left > (kDropRows - 1) * step ? kDropRows : (int)((left + step - 1) / step);   // rows to do
-    const T* xp = x + row0 * g.D + col;
-    T* yp = y + row0 * g.D + col;
-    RawPack<T, V> raw[kDropRows];
+  const uint32_t col = (uint32_t)pos * V;
+  const int64_t left = g.rows - row0, jump = step * g.D;
+  const int n = left <= 0 ? 0 : left > (kDropRows - 1) * step ? kDropRows : (int)((left + step - 1) / step);   // rows to do
+  const T* xp = x + row0 * g.D + col;
+  T* yp = y + row0 * g.D + col;
+  RawPack<T, V> raw[kDropRows];
 #pragma unroll
-    for (int r = 0; r < kDropRows; ++r)
-      if (r < n) raw[r] = ld_raw<T, V>(xp + r * jump);
-    const DropCol dc = drop_col(seed, col >> 3);
+  for (int r = 0; r < kDropRows; ++r)
+    if (r < n) raw[r] = ld_raw<T, V>(xp + r * jump);
+  const DropCol dc = drop_col(seed, col >> 3);
 #pragma unroll
-    for (int r = 0; r < kDropRows; ++r) {
-      if (r < n) {
-        float v[V];
+  for (int r = 0; r < kDropRows; ++r) {
+    if (r < n) {
+      float v[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = raw_get<V>(raw[r], e);
-        drop_apply<V>(drop, drop_bits<V>(seed, dc, drop_row(drop, seed, row0 + r * step), col), v);
-        PackIO<T, V>::store(yp + r * jump, v);
-      }
+      for (int e = 0; e < V; ++e) v[e] = raw_get<V>(raw[r], e);
+      drop_apply<V>(drop, drop_bits<V>(seed, dc, drop_row(drop, seed, row0 + r * step), col), v);
+      PackIO<T, V>::store(yp + r * jump, v);
     }
-  } else {
-    const int64_t col = (int64_t)pos * 8;
-    const DropCol dc = drop_col(seed, (uint32_t)pos);
+  }
+}
+
+// Rows that do not divide into packs: a warp owns 256 columns of kDropRows rows.  A lane computes the block of one group of
+// 8 columns, the warp exchanges the halves through shared memory of its own, and every access is to consecutive elements.
+template <typename T>
+__global__ void __launch_bounds__(256)
+k_counter_dropout_scalar(const T* __restrict__ x, T* __restrict__ y, DropGeo g, Drop drop) {
+  __shared__ uint4 exchange[8][32];
+  pdl_prologue();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t id = (int64_t)blockIdx.x * 8 + warp, chunk = id / g.CG;
+  const int col0 = (int)(id - chunk * g.CG) * 256;
+  const DropSeed seed = drop_seed(drop);
+  const DropCol dc = drop_col(seed, (uint32_t)(col0 >> 3) + lane);
+  for (int64_t row = chunk * kDropRows; row < min((chunk + 1) * kDropRows, g.rows); ++row) {   // uniform over the warp
+    const T* xp = x + row * g.D + col0 + lane;
+    T* yp = y + row * g.D + col0 + lane;
+    RawPack<T, 1> raw[8];
 #pragma unroll
-    for (int r = 0; r < kDropRows; ++r) {
-      const int64_t row = row0 + r * step, base = row * g.D + col;
-      if (row < g.rows) {
-        float v[8];
+    for (int k = 0; k < 8; ++k)
+      if (col0 + k * 32 + lane < g.D) raw[k] = ld_raw<T, 1>(xp + k * 32);
+    __syncwarp();
+    exchange[warp][lane] = drop_block(seed, dc, drop_row(drop, seed, row));
+    __syncwarp();
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(exchange[warp]) + lane;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = col + e < g.D ? to_f32(x[base + e]) : 0.f;
-        drop_apply<8>(drop, drop_bits<8>(seed, dc, drop_row(drop, seed, row), col), v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (col + e < g.D) y[base + e] = from_f32<T>(v[e]);
+    for (int k = 0; k < 8; ++k)
+      if (col0 + k * 32 + lane < g.D) {
+        DropBits<1> b;
+        b.w[0] = (uint32_t)h[k * 32] << 16;
+        float v[1] = {raw_get<1>(raw[k], 0)};
+        drop_apply<1>(drop, b, v);
+        yp[k * 32] = from_f32<T>(v[0]);
       }
-    }
   }
 }
 
@@ -105,7 +121,16 @@ extern "C" int mhc_counter_dropout(const void* x, const int64_t* rng, int drop_t
   DropGeo g;
   g.rows = rows;
   g.D = D;
-  g.groups = (int)(vec > 1 ? D / vec : (D + 7) / 8);
+  if (vec == 1) {
+    g.CG = (int)((D + 255) / 256);
+    const int64_t grid = ((rows + kDropRows - 1) / kDropRows * g.CG + 7) / 8;
+    if (grid > kMaxGridItems) return fail(MHC_ERR_BAD_SHAPE, "%s: too many work items (%lld)", what, (long long)grid);
+    ProfScope ps("k_counter_dropout", (cudaStream_t)stream);
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_counter_dropout_scalar<T>, (unsigned)grid, 256, 0, (cudaStream_t)stream, (const T*)x,
+                                       (T*)y, g, drop)));
+    return check_launch(what);
+  }
+  g.groups = (int)(D / vec);
   g.cols = g.groups >= 256 ? 256 : (g.groups + 31) / 32 * 32;
   g.sub = 256 / g.cols;
   g.CG = (g.groups + g.cols - 1) / g.cols;
@@ -114,7 +139,7 @@ extern "C" int mhc_counter_dropout(const void* x, const int64_t* rng, int drop_t
   cudaStream_t st = (cudaStream_t)stream;
   {
     ProfScope ps("k_counter_dropout", st);
-    MHC_DISPATCH(dtype, vec, (launch_k(k_counter_dropout<T, V>, (unsigned)grid, (unsigned)(g.cols * g.sub), 0, st,
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_counter_dropout<T, vec_width<T>::value>, (unsigned)grid, (unsigned)(g.cols * g.sub), 0, st,
                                        (const T*)x, (T*)y, g, drop)));
   }
   return check_launch(what);

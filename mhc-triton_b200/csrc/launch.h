@@ -53,6 +53,14 @@ int pick_vec(int dtype, int64_t D, std::initializer_list<const void*> ptrs);
     }                                                                                       \
   } while (0)
 
+// Runs CALL with T naming the element type.
+#define MHC_TYPE_DISPATCH(dtype, CALL)                             \
+  do {                                                             \
+    if ((dtype) == MHC_F32) { using T = float; CALL; }             \
+    else if ((dtype) == MHC_BF16) { using T = __nv_bfloat16; CALL; } \
+    else { using T = __half; CALL; }                               \
+  } while (0)
+
 // Programmatic dependent launch (on unless MHC_PDL=0 is set in the environment): every kernel of
 // this library may be scheduled while the previous kernel on the stream is still draining; each
 // kernel starts with griddepcontrol.wait, so it touches memory only after its predecessor has

@@ -10,6 +10,7 @@
 // backward's moves), but dweight keeps fp32 accuracy (from the rounded sums it is off by 1e-3).  Where the mix is
 // stored as branch_input, the stored value is what is normalised, so its backward, which reads it, is exact too.
 #include <algorithm>
+#include <atomic>
 
 #include "common.cuh"
 #include "launch.h"
@@ -38,6 +39,7 @@ struct NormFwd {
   int e8m0;
   float eps;
   float inv_D;
+  double inv_D64;
   Drop drop;
 };
 
@@ -80,27 +82,49 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return r;
 }
 
-// Scale of values whose largest magnitude is `amax`, and its reciprocal.  e8m0: the next power of two that is not
-// below amax / 448 (so nothing saturates), as its biased exponent: 448 = 1.75 * 2^8, so that is amax's exponent - 8, plus
-// one if its mantissa is above 1.75, which the carry of an integer addition says exactly; NaN and infinity become the
-// NaN code 255.  No division: a scale per 32 columns made IEEE divisions a tenth of the kernel.
-struct Scale { float inv; float f32; uint32_t code; };
-__device__ __forceinline__ Scale make_scale(float amax, int e8m0) {
+// Scale of the values u rstd whose largest |u| is `umax`, and the two factors that take u itself to e4m3.
+// fp32: scale = umax rstd / 448 and u (448 / umax): rstd cancels, so a quotient is two roundings from s w.
+// e8m0: the next power of two that is not below the largest |value| / 448 (so nothing saturates), as its biased
+// exponent: 448 = 1.75 * 2^8, so that is the value's exponent - 8, plus one if its mantissa is above 1.75, which the
+// carry of an integer addition says exactly; NaN and infinity become the NaN code 255.
+struct Scale { float f1, f2, f32; uint32_t code; };
+__device__ __forceinline__ Scale make_scale(float umax, double rstd, int e8m0) {
   Scale r;
+  r.f1 = (float)rstd;
   if (e8m0) {
-    const uint32_t b = __float_as_uint(amax);
+    const uint32_t b = __float_as_uint((float)((double)umax * rstd));
     const int e = (int)((b + 0x1fffffu) >> 23) - 8;
     const bool finite = b < 0x7f800000u;
     r.code = finite ? (uint32_t)(e < 1 ? 1 : e) : 255u;
     r.f32 = 0.f;   // not stored
-    r.inv = finite ? __uint_as_float((254u - r.code) << 23) : __int_as_float(0x7fc00000);
+    r.f2 = finite ? __uint_as_float((254u - r.code) << 23) : __int_as_float(0x7fc00000);
   } else {
-    const float s = amax * (1.f / kE4m3Max);
-    r.f32 = s < kMinScale ? kMinScale : s;  // false for NaN
-    r.inv = rcp_fast(r.f32);
+    const float s = (float)((double)umax * rstd * (1.0 / kE4m3Max));
     r.code = 0;
+    if (s < kMinScale) {  // false for NaN
+      r.f32 = kMinScale;
+      r.f2 = 8.50705917302346159e37f;   // 2^126
+    } else {
+      r.f32 = s;
+      r.f1 = __fdiv_rn(kE4m3Max, umax);
+      r.f2 = 1.f;
+    }
   }
   return r;
+}
+
+// 1 / sqrt(mean + eps) from a sum of squares: the hardware's approximation (2^-22.9) and one Newton step.
+__device__ __forceinline__ float row_rstd(float ss, float inv_D, float eps) {
+  const float x = fmaf(ss, inv_D, eps), r = rsqrtf(x);
+  return x > 1e-30f && x < 1e30f ? fmaf(0.5f * r, fmaf(-x * r, r, 1.f), r) : r;   // elsewhere the step itself would lose
+}
+// The same in fp64 for 8-bit outputs, where an error of the last fp32 bit moves a value or a power-of-two scale that is
+// next to a border to the other side (1 scale in 4 million at 16384 x 7168): five fp64 operations per thread and row.
+__device__ __forceinline__ double row_rstd64(float ss, double inv_D, float eps) {
+  const double x = (double)ss * inv_D + (double)eps;
+  const float f = rsqrtf((float)x);
+  const double r = (double)f;
+  return f > 1e-15f && f < 1e15f ? r + 0.5 * r * (1.0 - x * r * r) : r;
 }
 __device__ __forceinline__ void store_scale(void* scales, int64_t i, const Scale& s, int e8m0) {
   if (e8m0) ((uint8_t*)scales)[i] = (uint8_t)s.code;
@@ -169,20 +193,21 @@ k_norm_any_fwd(NormFwd a) {
     if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v * load_w<T>(a.weight, a.w_f32, d)));
   }
   block_sum_max<OUT == Out::RowScale>(ss, mx, sm);
-  const float rstd = rsqrtf(ss * a.inv_D + a.eps);
-  if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
   if constexpr (OUT == Out::Plain) {
+    const float rstd = row_rstd(ss, a.inv_D, a.eps);
+    if (a.rstd && threadIdx.x == 0) a.rstd[row] = rstd;
     for (int64_t d = threadIdx.x; d < D; d += 256)
       ((T*)a.y)[row * D + d] =
           from_f32<T>(src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d));
   } else if constexpr (OUT == Out::RowScale) {
-    const Scale s = make_scale(mx * rstd, a.e8m0);
+    const Scale s = make_scale(mx, row_rstd64(ss, a.inv_D64, a.eps), a.e8m0);
     if (threadIdx.x == 0) store_scale(a.scales, row, s, a.e8m0);
     for (int64_t d = threadIdx.x; d < D; d += 256) {
-      const float y = src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
-      ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y * s.inv, 0.f);
+      const float u = src_at<T, SRC, DROP>(a, seed, pre, row, d) * load_w<T>(a.weight, a.w_f32, d);
+      ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(u * s.f1 * s.f2, 0.f);
     }
   } else {  // a warp per group
+    const double rstd = row_rstd64(ss, a.inv_D64, a.eps);
     const int64_t G = (D + a.group - 1) / a.group;
     const int lane = threadIdx.x & 31;
     for (int64_t g = threadIdx.x >> 5; g < G; g += 8) {
@@ -192,17 +217,17 @@ k_norm_any_fwd(NormFwd a) {
         const int64_t d = g * a.group + j * 32 + lane;
         y[j] = 0.f;
         if (j * 32 < a.group && d < D)
-          y[j] = src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d);
+          y[j] = src_at<T, SRC, DROP>(a, seed, pre, row, d) * load_w<T>(a.weight, a.w_f32, d);
         m = max_nan(m, fabsf(y[j]));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const Scale s = make_scale(m, a.e8m0);
+      const Scale s = make_scale(m, rstd, a.e8m0);
       if (lane == 0) store_scale(a.scales, row * G + g, s, a.e8m0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int64_t d = g * a.group + j * 32 + lane;
-        if (j * 32 < a.group && d < D) ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y[j] * s.inv, 0.f);
+        if (j * 32 < a.group && d < D) ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(y[j] * s.f1 * s.f2, 0.f);
       }
     }
   }
@@ -275,16 +300,61 @@ k_norm_any_bwd(NormBwd a) {
 }
 
 // ------------------------------------------------------------------ rows that divide into 16-byte packs, in registers
-// A row belongs to `tpr` threads (a multiple of 32) that own the packs t, t + tpr, ...: NP packs each, all loaded
-// before the first use and kept in registers as fp32 between the row sum and the output, so the data is read once.
-// Narrow rows share a CTA of 256 threads.  Bound by memory; the one barrier of a row is covered by the other CTAs.
+// A row belongs to `tpr` threads (a multiple of 32) that own NP packs each, all loaded before the first use and kept in
+// registers as fp32 between the row sum and the output, so the data is read once.  Narrow rows share a CTA of 256
+// threads.  Bound by memory; the one barrier of a row is covered by the other CTAs.
+// Rows that do not divide into packs (odd widths, unaligned tensors) use the same kernels with packs of one element.
 struct RowMap {
   int tpr;   // threads per row
   int rpc;   // rows per CTA
   int DV;    // packs per row
 };
 
-// Row sum (and NaN-keeping maximum) over the warps of one row (16 at most); sm holds 2 x 16 floats.  One barrier.
+// The packs of thread t of a row: first, first + step, ...  Wide packs are spread over the row; single elements stay
+// within the warp's own 32 NP columns, whose dropout bits and groups of 64 or 128 columns are then the warp's affair.
+template <int V, int NP> struct Packs {
+  int first, step;
+  __device__ __forceinline__ Packs(int t, const RowMap& m)
+      : first(V > 1 ? t : (t >> 5) * 32 * NP + (t & 31)), step(V > 1 ? m.tpr : 32) {}
+};
+
+template <typename T, int V> __device__ __forceinline__ RawPack<T, V> raw_zero() {
+  RawPack<T, V> r;
+  if constexpr (V == 1) r.w = from_f32<T>(0.f);
+  else r.w = make_uint4(0, 0, 0, 0);
+  return r;
+}
+
+// Dropout bits of the thread's packs in one row.  With single elements a lane computes the block of one of the warp's 32
+// groups of 8 columns (NP = 8) and the warp exchanges the halves through 512 bytes of shared memory of its own.
+template <int V, int NP>
+__device__ __forceinline__ void drop_row_bits(const DropSeed& seed, const DropCol (&dcol)[V > 1 ? NP : 1], const DropRow& drow,
+                                              const Packs<V, NP>& pk, uint4* exchange, DropBits<V> (&bits)[NP]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) bits[k] = drop_bits<V>(seed, dcol[k], drow, (pk.first + k * pk.step) * V);
+  } else {
+    static_assert(NP == 8, "one block per lane");
+    uint4* mine = exchange + (threadIdx.x >> 5) * 32;
+    __syncwarp();
+    mine[threadIdx.x & 31] = drop_block(seed, dcol[0], drow);
+    __syncwarp();
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(mine) + (threadIdx.x & 31);
+#pragma unroll
+    for (int k = 0; k < NP; ++k) bits[k].w[0] = (uint32_t)h[k * 32] << 16;
+  }
+}
+template <int V, int NP>
+__device__ __forceinline__ void drop_cols(const DropSeed& seed, const Packs<V, NP>& pk, int t, DropCol (&dcol)[V > 1 ? NP : 1]) {
+  if constexpr (V > 1) {
+#pragma unroll
+    for (int k = 0; k < NP; ++k) dcol[k] = drop_col(seed, (uint32_t)((pk.first + k * pk.step) * V) >> 3);
+  } else {
+    dcol[0] = drop_col(seed, (uint32_t)t);   // t-th group of 8 columns of the row
+  }
+}
+
+// Row sum (and NaN-keeping maximum) over the warps of one row; sm holds 2 x 32 floats.  One barrier.
 template <bool MAX>
 __device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, const RowMap& m, int sub) {
 #pragma unroll
@@ -293,16 +363,16 @@ __device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, co
     if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
   if (m.tpr == 32) return;
-  const int warp = threadIdx.x >> 5, nw = m.tpr >> 5, l = threadIdx.x & 15;
+  const int warp = threadIdx.x >> 5, nw = m.tpr >> 5, l = threadIdx.x & 31;
   if ((threadIdx.x & 31) == 0) {
     sm[warp] = sum;
-    if (MAX) sm[16 + warp] = mx;
+    if (MAX) sm[32 + warp] = mx;
   }
   __syncthreads();
   sum = l < nw ? sm[sub * nw + l] : 0.f;
-  if (MAX) mx = l < nw ? sm[16 + sub * nw + l] : 0.f;
+  if (MAX) mx = l < nw ? sm[32 + sub * nw + l] : 0.f;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = 16; o > 0; o >>= 1) {
     sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (MAX) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   }
@@ -310,7 +380,9 @@ __device__ __forceinline__ void row_sum_max(float& sum, float& mx, float* sm, co
 
 template <typename T, int V>
 __device__ __forceinline__ void load_w_pack(const void* w, int w_f32, int col, float (&o)[V]) {
-  if (!w) {
+  if constexpr (V == 1) {
+    o[0] = load_w<T>(w, w_f32, col);
+  } else if (!w) {
 #pragma unroll
     for (int e = 0; e < V; ++e) o[e] = 1.f;
   } else if (w_f32) {
@@ -327,49 +399,76 @@ __device__ __forceinline__ void load_w_pack(const void* w, int w_f32, int col, f
   }
 }
 
-template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&y)[V], float inv) {
-  uint32_t w[V / 4];
+template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&u)[V], float f) {
+  if constexpr (V == 1) {
+    *p = (uint8_t)e4m3x2(u[0] * f, 0.f);
+  } else {
+    uint32_t w[V / 4];
 #pragma unroll
-  for (int i = 0; i < V / 4; ++i)
-    w[i] = (uint32_t)e4m3x2(y[4 * i] * inv, y[4 * i + 1] * inv) |
-           ((uint32_t)e4m3x2(y[4 * i + 2] * inv, y[4 * i + 3] * inv) << 16);
-  if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
-  else *reinterpret_cast<uint32_t*>(p) = w[0];
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = (uint32_t)e4m3x2(u[4 * i] * f, u[4 * i + 1] * f) | ((uint32_t)e4m3x2(u[4 * i + 2] * f, u[4 * i + 3] * f) << 16);
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint32_t*>(p) = w[0];
+  }
 }
 
 // From a row's values v (fp32), its sum of squares and, for a scale per row, its largest |v w| to the output: finishes the
 // sums over the row's threads (a barrier), then normalises, scales and stores.  `at` is the element offset of the thread's
 // first pack, DV the row's packs (0: the row does not exist).
 template <typename T, int V, int NP, Out OUT>
-__device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, float* sm, int sub, int t, int DV, int64_t row,
-                                          int64_t at, float (&v)[NP][V], const float (&w)[NP][V], float ss, float mx) {
-  const int stride = m.tpr * V;
+__device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, const Packs<V, NP>& pk, float* sm, int sub, int t,
+                                          int DV, int64_t row, int64_t at, float (&v)[NP][V], const float (&w)[NP][V],
+                                          float ss, float mx) {
+  const int stride = pk.step * V;
   row_sum_max<OUT == Out::RowScale>(ss, mx, sm, m, sub);
-  const float rstd = rsqrtf(ss * a.inv_D + a.eps);
-  if (a.rstd && DV && t == 0) a.rstd[row] = rstd;
-  Scale sc{};
-  if constexpr (OUT == Out::RowScale) {
-    sc = make_scale(mx * rstd, a.e8m0);
-    if (DV && t == 0) store_scale(a.scales, row, sc, a.e8m0);
-  }
-  const int lanes = OUT == Out::GroupScale ? a.group / V : 1;          // group / V consecutive packs = consecutive lanes
-  const int G = OUT == Out::GroupScale ? ((int)a.D + a.group - 1) / a.group : 1;
+  if constexpr (OUT == Out::Plain) {
+    const float rstd = row_rstd(ss, a.inv_D, a.eps);
+    if (a.rstd && DV && t == 0) a.rstd[row] = rstd;
 #pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int p = t + k * m.tpr;
+    for (int k = 0; k < NP; ++k) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * rstd * w[k][e];
-    if constexpr (OUT == Out::GroupScale) {
-      float g = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e) g = max_nan(g, fabsf(v[k][e]));
-      for (int o = lanes >> 1; o > 0; o >>= 1) g = max_nan(g, __shfl_xor_sync(0xffffffffu, g, o));
-      sc = make_scale(g, a.e8m0);
-      if (p < DV && (p & (lanes - 1)) == 0) store_scale(a.scales, row * G + (uint32_t)p / (uint32_t)lanes, sc, a.e8m0);
+      for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * rstd * w[k][e];
+      if (pk.first + k * pk.step < DV) PackIO<T, V>::store((T*)a.y + at + k * stride, v[k]);
     }
-    if (p < DV) {
-      if constexpr (OUT == Out::Plain) PackIO<T, V>::store((T*)a.y + at + k * stride, v[k]);
-      else store_e4m3<V>((uint8_t*)a.y + at + k * stride, v[k], sc.inv);
+  } else {
+    const double rstd = row_rstd64(ss, a.inv_D64, a.eps);
+    Scale sc{};
+    float g[NP];   // largest |v w| of the group a pack is in
+    if constexpr (OUT == Out::RowScale) {
+      sc = make_scale(mx, rstd, a.e8m0);
+      if (DV && t == 0) store_scale(a.scales, row, sc, a.e8m0);
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      g[k] = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[k][e] *= w[k][e];
+        if (OUT == Out::GroupScale) g[k] = max_nan(g[k], fabsf(v[k][e]));
+      }
+    }
+    const int lanes = V > 1 ? a.group / V : 32;   // consecutive lanes that share a group
+    const int G = OUT == Out::GroupScale ? ((int)a.D + a.group - 1) / a.group : 1;
+    if constexpr (OUT == Out::GroupScale && V == 1) {   // 64 or 128 columns are 2 or 4 consecutive k of the warp
+#pragma unroll
+      for (int k = 0; k < NP; k += 2)
+        if (a.group >= 64) g[k] = g[k + 1] = max_nan(g[k], g[k + 1]);
+#pragma unroll
+      for (int k = 0; k < NP; k += 4)
+        if (a.group >= 128) g[k] = g[k + 1] = g[k + 2] = g[k + 3] = max_nan(g[k], g[k + 2]);
+    }
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int p = pk.first + k * pk.step;
+      if constexpr (OUT == Out::GroupScale) {
+        for (int o = lanes >> 1; o > 0; o >>= 1) g[k] = max_nan(g[k], __shfl_xor_sync(0xffffffffu, g[k], o));
+        sc = make_scale(g[k], rstd, a.e8m0);
+        if (p < DV && (p * V & (a.group - 1)) == 0)
+          store_scale(a.scales, row * G + (uint32_t)(p * V) / (uint32_t)a.group, sc, a.e8m0);
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[k][e] *= sc.f1;
+      if (p < DV) store_e4m3<V>((uint8_t*)a.y + at + k * stride, v[k], sc.f2);
     }
   }
 }
@@ -392,24 +491,26 @@ __device__ __forceinline__ void mix_pack(const RawPack<T, V> (&x)[4], const floa
            pre[3] * raw_get<V>(x[3], e);
 }
 
-// One row per thread group, once: few rows.
+// One row per thread group, once.
 template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
-__global__ void __launch_bounds__(512, NP == 2 ? 2 : 1)
+__global__ void __launch_bounds__(V == 1 ? 1024 : 512, NP == 2 ? 2 : 1)
 k_norm_fwd(NormFwd a, RowMap m) {
   pdl_prologue();
-  __shared__ float sm[32];
+  __shared__ float sm[64];
+  __shared__ uint4 exchange[DROP && V == 1 ? 1024 : 1];
   const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
-  const int64_t row = (int64_t)blockIdx.x * m.rpc + sub, D = a.D, at = row * D + t * V;
-  const int DV = row < a.rows ? m.DV : 0, stride = m.tpr * V;   // a row past the end owns no packs
+  const Packs<V, NP> pk(t, m);
+  const int64_t row = (int64_t)blockIdx.x * m.rpc + sub, D = a.D, at = row * D + pk.first * V;
+  const int DV = row < a.rows ? m.DV : 0, stride = pk.step * V;   // a row past the end owns no packs
   constexpr int NS = SRC == Src::Mix ? 4 : 2;
-  const T* xp = (const T*)a.x + (SRC == Src::Mix ? 4 : 1) * row * D + t * V;
+  const T* xp = (const T*)a.x + (SRC == Src::Mix ? 4 : 1) * row * D + pk.first * V;
   const T* rp = (const T*)a.res + at;
   RawPack<T, V> raw[NP][NS];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
 #pragma unroll
-    for (int n = 0; n < NS; ++n) raw[k][n].w = make_uint4(0, 0, 0, 0);
-    if (t + k * m.tpr < DV) {
+    for (int n = 0; n < NS; ++n) raw[k][n] = raw_zero<T, V>();
+    if (pk.first + k * pk.step < DV) {
       if constexpr (SRC == Src::Mix) {
 #pragma unroll
         for (int n = 0; n < 4; ++n) raw[k][n] = ld_raw<T, V>(xp + n * D + k * stride);
@@ -432,29 +533,27 @@ k_norm_fwd(NormFwd a, RowMap m) {
   for (int k = 0; k < NP; ++k) {
 #pragma unroll
     for (int e = 0; e < V; ++e) w[k][e] = 0.f;
-    if (t + k * m.tpr < DV) load_w_pack<T, V>(a.weight, a.w_f32, t * V + k * stride, w[k]);
+    if (pk.first + k * pk.step < DV) load_w_pack<T, V>(a.weight, a.w_f32, pk.first * V + k * stride, w[k]);
   }
-  DropSeed seed{};
-  DropRow drow{};
+  DropBits<V> bits[NP];
   if constexpr (DROP) {
-    seed = drop_seed(a.drop);
-    drow = drop_row(a.drop, seed, row);
+    const DropSeed seed = drop_seed(a.drop);
+    DropCol dcol[V > 1 ? NP : 1];
+    drop_cols<V, NP>(seed, pk, t, dcol);
+    drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, exchange, bits);
   }
   T* so = (T*)a.sum_out + at;
   float v[NP][V], ss = 0.f, mx = 0.f;
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    const bool ok = t + k * m.tpr < DV;
+    const bool ok = pk.first + k * pk.step < DV;
     if constexpr (SRC == Src::Mix) {
       mix_pack<T, V>(raw[k], pre, v[k]);
       if (a.sum_out && ok) PackIO<T, V>::store_round(so + k * stride, v[k]);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] = raw_get<V>(raw[k][0], e);
-      if constexpr (DROP) {
-        const int col = t * V + k * stride;
-        drop_apply<V>(a.drop, drop_bits<V>(seed, drop_col(seed, (uint32_t)col >> 3), drow, col), v[k]);
-      }
+      if constexpr (DROP) drop_apply<V>(a.drop, bits[k], v[k]);
       if (a.res) {
 #pragma unroll
         for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(raw[k][1], e);
@@ -463,21 +562,22 @@ k_norm_fwd(NormFwd a, RowMap m) {
     }
     norm_gather<V, OUT>(v[k], w[k], ss, mx);
   }
-  norm_emit<T, V, NP, OUT>(a, m, sm, sub, t, DV, row, at, v, w, ss, mx);
+  norm_emit<T, V, NP, OUT>(a, m, pk, sm, sub, t, DV, row, at, v, w, ss, mx);
 }
 
-// Many rows: persistent CTAs that keep the weight and the columns' part of the generator in registers, with the next row's
+// Many rows and more to do per pack than to add, norm and store it (8-bit output, dropout): persistent CTAs that keep the weight and the columns' part of the generator in registers, with the next row's
 // packs on the way by cp.async into slots of shared memory that only the thread itself reads.
 template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
 __global__ void __launch_bounds__(512, 2)
 k_norm_fwd_ring(NormFwd a, RowMap m) {
   extern __shared__ __align__(16) uint4 ring[];   // [2][NP][NS][threads]
-  __shared__ float sm[2][32];
+  __shared__ float sm[2][64];
   pdl_prologue();
   constexpr int NS = SRC == Src::Mix ? 4 : 2;
   const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
+  const Packs<V, NP> pk(t, m);
   const int64_t D = a.D;
-  const int stride = m.tpr * V;
+  const int stride = pk.step * V;
   const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16u, pitch = blockDim.x * 16u;
   const uint32_t rows = (uint32_t)a.rows, step = gridDim.x * m.rpc;   // at most 2^31 rows
   auto issue = [&](int stage, uint32_t row) {
@@ -508,12 +608,11 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
   uint32_t row = blockIdx.x * m.rpc + sub;
   issue(0, row);
   DropSeed seed{};
-  DropCol dcol[DROP ? NP : 1];
+  DropCol dcol[NP];
   float w[NP][V];
-  if constexpr (DROP) seed = drop_seed(a.drop);
+  if constexpr (DROP) drop_cols<V, NP>(seed = drop_seed(a.drop), pk, t, dcol);
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
-    if constexpr (DROP) dcol[k] = drop_col(seed, (uint32_t)(t * V + k * stride) >> 3);
 #pragma unroll
     for (int e = 0; e < V; ++e) w[k][e] = 0.f;
     if (t + k * m.tpr < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, t * V + k * stride, w[k]);
@@ -531,12 +630,9 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
         for (int n = 0; n < 4; ++n) pre[n] = __ldg(h + n);
       }
     }
-    DropBits<V> bits[DROP ? NP : 1];
-    if constexpr (DROP) {   // while the row is on its way
-      const DropRow drow = drop_row(a.drop, seed, row);
-#pragma unroll
-      for (int k = 0; k < NP; ++k) bits[k] = drop_bits<V>(seed, dcol[k], drow, t * V + k * stride);
-    }
+    DropBits<V> bits[NP];
+    if constexpr (DROP)   // while the row is on its way
+      drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, nullptr, bits);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     float v[NP][V], ss = 0.f, mx = 0.f;
 #pragma unroll
@@ -565,7 +661,7 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
         norm_gather<V, OUT>(v[k], w[k], ss, mx);
       }
     }
-    norm_emit<T, V, NP, OUT>(a, m, sm[stage], sub, t, DV, row, at, v, w, ss, mx);
+    norm_emit<T, V, NP, OUT>(a, m, pk, sm[stage], sub, t, DV, row, at, v, w, ss, mx);
     stage ^= 1;   // the next row's sums go to the other half of sm: nobody can still be reading it
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -575,32 +671,30 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
 // dweight's running sums in registers.  The packs of the next DEPTH - 1 rows are on the way meanwhile, by cp.async into
 // slots of shared memory that only the thread itself reads (no barrier): in registers they spilled, and the
 // stream form ran at 42 % of the memory's rate.  An item is rpc rows (Add) or a chunk of a batch element's tokens
-// (Mix), walked rpc abreast.
-template <typename T, int V, int NP, int DEPTH, Src SRC, bool DROP>
-__global__ void __launch_bounds__(512)
+// (Mix), walked rpc abreast.  DEPTH 0 (single elements, which cp.async cannot copy): loads straight from memory.
+template <typename T, int V, int NP, int DEPTH, int THREADS, Src SRC, bool DROP>
+__global__ void __launch_bounds__(THREADS)
 k_norm_bwd(NormBwd a, RowMap m) {
   extern __shared__ __align__(16) uint4 ring[];   // [DEPTH][NP][NS][threads]
-  __shared__ float sm[2][32];
-  __shared__ float red[16 * 4];
+  __shared__ float sm[2][64];
+  __shared__ float red[32 * 4];
+  __shared__ uint4 exchange[DROP && V == 1 ? 1024 : 1];
   pdl_prologue();
   constexpr int NS = SRC == Src::Mix ? 5 : 4;   // Mix: dy, H[0..3]; Add: dy, x, residual, dsum
   const int sub = m.rpc == 1 ? 0 : threadIdx.x / m.tpr, t = threadIdx.x - sub * m.tpr;
+  const Packs<V, NP> pk(t, m);
   const int64_t D = a.D;
-  const int stride = m.tpr * V;
+  const int stride = pk.step * V;
   const uint32_t mine = (uint32_t)__cvta_generic_to_shared(ring) + threadIdx.x * 16u, pitch = blockDim.x * 16u;
   DropSeed seed{};
-  DropCol dcol[DROP ? NP : 1];
-  if constexpr (DROP) {
-    seed = drop_seed(a.drop);
-#pragma unroll
-    for (int k = 0; k < NP; ++k) dcol[k] = drop_col(seed, (uint32_t)(t * V + k * stride) >> 3);
-  }
+  DropCol dcol[V > 1 ? NP : 1];
+  if constexpr (DROP) drop_cols<V, NP>(seed = drop_seed(a.drop), pk, t, dcol);
   float w[NP][V], dw[NP][V];
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[k][e] = w[k][e] = 0.f;
-    if (t + k * m.tpr < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, t * V + k * stride, w[k]);
+    if (pk.first + k * pk.step < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, pk.first * V + k * stride, w[k]);
   }
 
   // where the CTA is: rows base .. base + rpc - 1 of the item, the item's end
@@ -629,19 +723,20 @@ k_norm_bwd(NormBwd a, RowMap m) {
     float rstd = 0.f;
     if (q.item < a.items && row < q.end) {
       rstd = __ldg(a.rstd + row);
+      if constexpr (DEPTH == 0) return rstd;
       const T* src[NS];
-      src[0] = (const T*)a.dy + row * D + t * V;
+      src[0] = (const T*)a.dy + row * D + pk.first * V;
       if constexpr (SRC == Src::Mix) {
 #pragma unroll
-        for (int n = 0; n < 4; ++n) src[1 + n] = (const T*)a.x + (row * 4 + n) * D + t * V;
+        for (int n = 0; n < 4; ++n) src[1 + n] = (const T*)a.x + (row * 4 + n) * D + pk.first * V;
       } else {
-        src[1] = (const T*)a.x + row * D + t * V;
-        src[2] = (const T*)a.res + row * D + t * V;
-        src[3] = (const T*)a.dsum + row * D + t * V;
+        src[1] = (const T*)a.x + row * D + pk.first * V;
+        src[2] = (const T*)a.res + row * D + pk.first * V;
+        src[3] = (const T*)a.dsum + row * D + pk.first * V;
       }
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        if (t + k * m.tpr < m.DV) {
+        if (pk.first + k * pk.step < m.DV) {
 #pragma unroll
           for (int n = 0; n < NS; ++n)
             if (SRC == Src::Mix || n < 2 || (n == 2 ? a.res : a.dsum))
@@ -650,16 +745,23 @@ k_norm_bwd(NormBwd a, RowMap m) {
                            : "memory");
         }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if constexpr (DEPTH > 0) asm volatile("cp.async.commit_group;" ::: "memory");
     return rstd;
   };
-  auto slot = [&](int stage, int k, int n) -> RawPack<T, V> {
-    RawPack<T, V> r;
-    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r.w.x), "=r"(r.w.y), "=r"(r.w.z), "=r"(r.w.w)
-                 : "r"(mine + (uint32_t)((stage * NP + k) * NS + n) * pitch)
-                 : "memory");
-    return r;
+  auto slot = [&](int stage, int k, int n, int64_t row) -> RawPack<T, V> {
+    if constexpr (DEPTH == 0) {
+      const T* src = n == 0 ? (const T*)a.dy + row * D
+                   : SRC == Src::Mix ? (const T*)a.x + (row * 4 + n - 1) * D
+                   : (const T*)(n == 1 ? a.x : n == 2 ? a.res : a.dsum) + row * D;
+      return ld_raw<T, V>(src + pk.first * V + k * stride);
+    } else {
+      RawPack<T, V> r;
+      asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                   : "=r"(r.w.x), "=r"(r.w.y), "=r"(r.w.z), "=r"(r.w.w)
+                   : "r"(mine + (uint32_t)((stage * NP + k) * NS + n) * pitch)
+                   : "memory");
+      return r;
+    }
   };
 
   float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -676,22 +778,32 @@ k_norm_bwd(NormBwd a, RowMap m) {
   }
   while (q.item < a.items) {
     float rstd;
-    if constexpr (DEPTH == 1) {
+    if constexpr (DEPTH <= 1) {
       rstd = issue(0, q);
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      if (DEPTH == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
       rstd = ahead[0];
 #pragma unroll
       for (int d = 0; d + 1 < DEPTH - 1; ++d) ahead[d] = ahead[d + 1];
       ahead[DEPTH - 2] = issue(stage == 0 ? DEPTH - 1 : stage - 1, qi);   // the stage read in the previous iteration
       qi = next(qi);
-      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH > 0 ? DEPTH - 1 : 0) : "memory");
     }
     const int64_t row = q.base + sub;
     const int DV = row < q.end ? m.DV : 0;
     const Pos q2 = next(q);
-    DropRow drow{};
-    if constexpr (DROP) drow = drop_row(a.drop, seed, row);
+    RawPack<T, V> now[DEPTH == 0 ? NP : 1][3];   // dy, x, residual: all loads before the warp meets over the bits
+    if constexpr (DEPTH == 0 && SRC == Src::Add) {
+#pragma unroll
+      for (int k = 0; k < NP; ++k)
+        if (pk.first + k * pk.step < DV) {
+          now[k][0] = slot(0, k, 0, row);
+          now[k][1] = slot(0, k, 1, row);
+          if (a.res) now[k][2] = slot(0, k, 2, row);
+        }
+    }
+    DropBits<V> bits[DROP ? NP : 1];
+    if constexpr (DROP) drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, exchange, bits);
     if constexpr (SRC == Src::Mix) {
       if (q.item != pre_of) {
         pre_of = q.item;
@@ -700,31 +812,24 @@ k_norm_bwd(NormBwd a, RowMap m) {
       }
     }
     float s[NP][V], h[NP][V], c = 0.f, unused = 0.f;
-    DropBits<V> bits[DROP ? NP : 1];
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
 #pragma unroll
       for (int e = 0; e < V; ++e) s[k][e] = h[k][e] = 0.f;
-      if (t + k * m.tpr < DV) {
-        const RawPack<T, V> dy = slot(stage, k, 0);
+      if (pk.first + k * pk.step < DV) {
+        const RawPack<T, V> dy = DEPTH == 0 && SRC == Src::Add ? now[DEPTH == 0 ? k : 0][0] : slot(stage, k, 0, row);
         if constexpr (SRC == Src::Mix) {
           RawPack<T, V> x[4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) x[n] = slot(stage, k, 1 + n);
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            s[k][e] = ((pre[0] * raw_get<V>(x[0], e) + pre[1] * raw_get<V>(x[1], e)) + pre[2] * raw_get<V>(x[2], e)) +
-                      pre[3] * raw_get<V>(x[3], e);
+          for (int n = 0; n < 4; ++n) x[n] = slot(stage, k, 1 + n, row);
+          mix_pack<T, V>(x, pre, s[k]);
         } else {
-          const RawPack<T, V> x = slot(stage, k, 1);
+          const RawPack<T, V> x = DEPTH == 0 ? now[DEPTH == 0 ? k : 0][1] : slot(stage, k, 1, row);
 #pragma unroll
           for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(x, e);
-          if constexpr (DROP) {
-            bits[k] = drop_bits<V>(seed, dcol[k], drow, t * V + k * stride);
-            drop_apply<V>(a.drop, bits[k], s[k]);
-          }
+          if constexpr (DROP) drop_apply<V>(a.drop, bits[k], s[k]);
           if (a.res) {
-            const RawPack<T, V> r = slot(stage, k, 2);
+            const RawPack<T, V> r = DEPTH == 0 ? now[DEPTH == 0 ? k : 0][2] : slot(stage, k, 2, row);
 #pragma unroll
             for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r, e);
           }
@@ -743,15 +848,15 @@ k_norm_bwd(NormBwd a, RowMap m) {
     const float kk = c * rstd * rstd * rstd * a.inv_D;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      if (t + k * m.tpr < DV) {
+      if (pk.first + k * pk.step < DV) {
         float g[V];
 #pragma unroll
         for (int e = 0; e < V; ++e) g[e] = rstd * h[k][e] - s[k][e] * kk;
         if constexpr (SRC == Src::Mix) {
-          T* o = (T*)a.dx + row * 4 * D + t * V + k * stride;
+          T* o = (T*)a.dx + row * 4 * D + pk.first * V + k * stride;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const RawPack<T, V> x = slot(stage, k, 1 + n);
+            const RawPack<T, V> x = slot(stage, k, 1 + n, row);
             float u[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -762,15 +867,15 @@ k_norm_bwd(NormBwd a, RowMap m) {
           }
         } else {
           if (a.dsum) {
-            const RawPack<T, V> ds = slot(stage, k, 3);
+            const RawPack<T, V> ds = slot(stage, k, 3, row);
 #pragma unroll
             for (int e = 0; e < V; ++e) g[e] += raw_get<V>(ds, e);
           }
           if constexpr (DROP) {
-            if (a.dres) PackIO<T, V>::store((T*)a.dres + row * D + t * V + k * stride, g);
+            if (a.dres) PackIO<T, V>::store((T*)a.dres + row * D + pk.first * V + k * stride, g);
             drop_apply<V>(a.drop, bits[k], g);
           }
-          PackIO<T, V>::store((T*)a.dx + row * D + t * V + k * stride, g);
+          PackIO<T, V>::store((T*)a.dx + row * D + pk.first * V + k * stride, g);
         }
       }
     }
@@ -783,17 +888,19 @@ k_norm_bwd(NormBwd a, RowMap m) {
       }
     }
     q = q2;
-    stage = stage + 1 == DEPTH ? 0 : stage + 1;
+    stage = stage + 1 >= DEPTH ? 0 : stage + 1;
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (a.dw_part) {
-    float* o = a.dw_part + ((int64_t)blockIdx.x * m.rpc + sub) * D + t * V;
+    float* o = a.dw_part + ((int64_t)blockIdx.x * m.rpc + sub) * D + pk.first * V;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      if (t + k * m.tpr < m.DV) {
+      if (pk.first + k * pk.step < m.DV) {
 #pragma unroll
-        for (int e = 0; e < V; e += 4)
-          *reinterpret_cast<float4*>(o + k * stride + e) = make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]);
+        for (int e = 0; e < V; e += 4) {
+          if constexpr (V == 1) o[k * stride] = dw[k][0];
+          else *reinterpret_cast<float4*>(o + k * stride + e) = make_float4(dw[k][e], dw[k][e + 1], dw[k][e + 2], dw[k][e + 3]);
+        }
       }
     }
   }
@@ -864,23 +971,32 @@ static int64_t mix_chunks(int64_t S, int rpc) { return (S + mix_tpc(S, rpc) - 1)
 // Shared memory of an SM that the resident CTAs' rings may use together (each has a few hundred bytes of its own beside).
 constexpr size_t kRingBytes = 224 * 1024;
 
-// launch_k for a kernel whose dynamic shared memory may exceed the 48 KiB it gets without asking .
-template <typename... KArgs, typename... Args>
-static void launch_ring(void (*kernel)(KArgs...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {
-  if (smem > 48 * 1024) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  launch_k(kernel, grid, block, smem, st, std::forward<Args>(args)...);
+// launch_k for a kernel whose dynamic shared memory may exceed the 48 KiB, static included, it gets without asking.
+template <auto Kernel, typename... Args>
+static void launch_ring(unsigned grid, unsigned block, size_t smem, cudaStream_t st, Args&&... args) {
+  static std::atomic<uint32_t> asked{0};   // devices on which the attribute is set
+  int dev = 0;
+  if (smem > 40 * 1024 && cudaGetDevice(&dev) == cudaSuccess && (dev > 31 || !(asked.load() >> dev & 1))) {
+    (void)cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRingBytes);
+    if (dev < 32) asked.fetch_or(1u << dev);
+  }
+  launch_k(Kernel, grid, block, smem, st, std::forward<Args>(args)...);
 }
 
 // Threads and rows per CTA for rows of D elements in packs of V: `np` packs per thread.
 static RowMap row_map(int64_t D, int V, int np) {
   RowMap m;
   m.DV = (int)(D / V);
-  m.tpr = ((m.DV + np - 1) / np + 31) / 32 * 32;
+  m.tpr = V > 1 ? ((m.DV + np - 1) / np + 31) / 32 * 32 : (m.DV + 32 * np - 1) / (32 * np) * 32;
   m.rpc = m.tpr <= 128 ? 256 / m.tpr : 1;
   return m;
 }
-// Packs per thread of the register kernels: 2 up to 1024 packs per row, 4 up to 2048; 0: the row does not fit.
-static int packs_per_thread(int64_t D, int V) { return D / V <= 1024 ? 2 : D / V <= 2048 ? 4 : 0; }
+// Packs per thread of the register kernels: 2 up to 1024 packs per row, 4 up to 2048; 8 single elements up to 8192;
+// 0: the row does not fit.
+static int packs_per_thread(int64_t D, int V) {
+  if (V == 1) return D <= 8192 ? 8 : 0;
+  return D / V <= 1024 ? 2 : D / V <= 2048 ? 4 : 0;
+}
 
 // Scratch: at most two rows' worth of partial sums per SM and row walked abreast (rpc <= 8, and then D <= 512), plus the
 // chunks' dH_pre sums.
@@ -892,13 +1008,6 @@ int64_t rms_norm_bwd_scratch_bytes(int64_t rows, int64_t D) {
 int64_t stream_norm_bwd_scratch_bytes(int64_t B, int64_t S, int64_t D) {
   return (dw_rows(D) * D + B * mix_chunks(S, 1) * 4 + 4) * (int64_t)sizeof(float);
 }
-
-#define MHC_TYPE_DISPATCH(dtype, CALL)                             \
-  do {                                                             \
-    if ((dtype) == MHC_F32) { using T = float; CALL; }             \
-    else if ((dtype) == MHC_BF16) { using T = __nv_bfloat16; CALL; } \
-    else { using T = __half; CALL; }                               \
-  } while (0)
 
 // Arguments common to all entry points of this file.
 static int check_norm(const char* what, int64_t rows, int64_t D, int dtype, const void* weight, int wdtype) {
@@ -921,7 +1030,7 @@ template <Src SRC, bool DROP, Out OUT>
 static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_t st) {
   ProfScope ps(SRC == Src::Mix ? "k_stream_norm_fwd" : "k_rms_norm_fwd", st);
   const int vec = pick_vec(dtype, a.D, {a.x, a.res, a.weight, a.sum_out, a.y});
-  const int np = vec > 1 ? packs_per_thread(a.D, vec) : 0;
+  const int np = packs_per_thread(a.D, vec);
   if (np == 0) {
     MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_fwd<T, SRC, DROP, OUT>, (unsigned)a.rows, 256, 0, st, a)));
     return check_launch(what);
@@ -931,11 +1040,12 @@ static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_
   const size_t smem = (size_t)2 * block * np * (SRC == Src::Mix ? 4 : 2) * 16;
   const int per_sm = std::min(1024 / (int)block, (int)(kRingBytes / smem));
   if ((DROP || OUT != Out::Plain) && np == 2 && per_sm > 0 && grid >= (unsigned)(MHC_RING_MIN * per_sm * sm_count())) {
-    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_fwd_ring<T, vec_width<T>::value, 2, SRC, DROP, OUT>, (unsigned)(per_sm * sm_count()),
+    MHC_TYPE_DISPATCH(dtype, (launch_ring<k_norm_fwd_ring<T, vec_width<T>::value, 2, SRC, DROP, OUT>>((unsigned)(per_sm * sm_count()),
                                           block, smem, st, a, m)));
     return check_launch(what);
   }
-  if (np == 2) MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, vec_width<T>::value, 2, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
+  if (vec == 1) MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, 1, 8, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
+  else if (np == 2) MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, vec_width<T>::value, 2, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
   else MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_fwd<T, vec_width<T>::value, 4, SRC, DROP, OUT>, grid, block, 0, st, a, m)));
   return check_launch(what);
 }
@@ -946,7 +1056,7 @@ template <Src SRC, bool DROP>
 static int launch_bwd(const char* what, NormBwd& a, float* scratch, int dtype, cudaStream_t st) {
   ProfScope ps(SRC == Src::Mix ? "k_stream_norm_bwd" : "k_rms_norm_bwd", st);
   const int vec = pick_vec(dtype, a.D, {a.dy, a.dsum, a.x, a.res, a.weight, a.dx, a.dres});
-  const int np = vec > 1 ? packs_per_thread(a.D, vec) : 0;
+  const int np = packs_per_thread(a.D, vec);
   RowMap m{256, 1, 0};
   if (np) m = row_map(a.D, vec, np);
   if constexpr (SRC == Src::Mix) {
@@ -966,10 +1076,14 @@ static int launch_bwd(const char* what, NormBwd& a, float* scratch, int dtype, c
   const size_t stage = (size_t)threads * np * (SRC == Src::Mix ? 5 : 4) * 16;
   if (np == 0)
     MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_any_bwd<T, SRC, DROP>, (unsigned)ctas, 256, 0, st, a)));
+  else if (vec == 1 && threads <= 512)
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, 1, 8, 0, 512, SRC, DROP>, (unsigned)ctas, threads, 0, st, a, m)));
+  else if (vec == 1)
+    MHC_TYPE_DISPATCH(dtype, (launch_k(k_norm_bwd<T, 1, 8, 0, 1024, SRC, DROP>, (unsigned)ctas, threads, 0, st, a, m)));
   else if (np == 4)
-    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_bwd<T, vec_width<T>::value, 4, 1, SRC, DROP>, (unsigned)ctas, threads, stage, st, a, m)));
+    MHC_TYPE_DISPATCH(dtype, (launch_ring<k_norm_bwd<T, vec_width<T>::value, 4, 1, 512, SRC, DROP>>((unsigned)ctas, threads, stage, st, a, m)));
   else   // three stages: 229 instead of 207 us at 32768 x 4096 bf16
-    MHC_TYPE_DISPATCH(dtype, (launch_ring(k_norm_bwd<T, vec_width<T>::value, 2, 2, SRC, DROP>, (unsigned)ctas, threads, 2 * stage, st, a, m)));
+    MHC_TYPE_DISPATCH(dtype, (launch_ring<k_norm_bwd<T, vec_width<T>::value, 2, 2, 512, SRC, DROP>>((unsigned)ctas, threads, 2 * stage, st, a, m)));
   return check_launch(what);
 }
 
@@ -989,7 +1103,7 @@ int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, 
                          float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st) {
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = wdtype == MHC_F32; a.sum_out = bi; a.y = y; a.rstd = rstd;
-  a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
+  a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
   return launch_fwd<Src::Mix, false, Out::Plain>("stream_norm_fwd", a, dtype, st);
 }
 
@@ -1010,7 +1124,7 @@ extern "C" int mhc_add_rms_norm_fwd(const void* x, const void* residual, const v
   if (rows == 0 || D == 0) return MHC_OK;
   if (!x || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = y;
-  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
+  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
   cudaStream_t st = (cudaStream_t)stream;
   return drop ? launch_fwd<Src::Add, true, Out::Plain>(what, a, dtype, st)
               : launch_fwd<Src::Add, false, Out::Plain>(what, a, dtype, st);
@@ -1028,7 +1142,7 @@ extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, c
   NormFwd a{};
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = q;
   a.scales = scales; a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0;
-  a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
+  a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Add, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Add, false, Out::RowScale>(what, a, dtype, st);
@@ -1091,7 +1205,7 @@ extern "C" int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, cons
   if (!H || !H_pre || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q; a.scales = scales;
-  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D = (float)(1.0 / (double)D);
+  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Mix, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Mix, false, Out::RowScale>(what, a, dtype, st);

@@ -106,6 +106,39 @@ __device__ __forceinline__ DropBits<V> drop_bits(const DropSeed& s, const DropCo
   return o;
 }
 
+// The bits of a thread that stays in the V columns from `col` on and walks the rows row, row + step, ...  With single
+// columns the 8 lanes of a group of columns each compute the block of one of the next 8 rows and hand the words round:
+// one block per 8 elements, as with packs.  The warp must walk together then, lanes past the last column included.
+template <int V> struct DropWalk {
+  DropSeed seed;
+  DropCol col;
+  uint4 block;
+  int used;
+  __device__ __forceinline__ void start(const DropSeed& s, int64_t c0) {
+    seed = s;
+    col = drop_col(s, (uint32_t)(c0 >> 3));
+    used = 8;
+  }
+  __device__ __forceinline__ DropBits<V> bits(const Drop& d, int64_t row, int64_t step, int64_t c0) {
+    if constexpr (V > 1) {
+      return drop_bits<V>(seed, col, drop_row(d, seed, row), c0);
+    } else {
+      const int lane = threadIdx.x & 31;
+      if (used == 8) {
+        block = drop_block(seed, col, drop_row(d, seed, row + (lane & 7) * step));
+        used = 0;
+      }
+      const int from = (lane & 24) | used++;
+      const uint32_t x = __shfl_sync(0xffffffffu, block.x, from), y = __shfl_sync(0xffffffffu, block.y, from);
+      const uint32_t z = __shfl_sync(0xffffffffu, block.z, from), w = __shfl_sync(0xffffffffu, block.w, from);
+      const uint32_t lo = (lane & 2) ? y : x, hi = (lane & 2) ? w : z, word = (lane & 4) ? hi : lo;
+      DropBits<1> o;
+      o.w[0] = (lane & 1) ? word : word << 16;
+      return o;
+    }
+  }
+};
+
 // v[e] -> 0 where dropped (whatever v held, infinities and NaN included), v * scale where kept.
 template <int V>
 __device__ __forceinline__ void drop_apply(const Drop& d, const DropBits<V>& b, float (&v)[V]) {

@@ -205,17 +205,19 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
   pdl_prologue();
   extern __shared__ __align__(16) float sm[];   // DROP: the ring
   const Item it = decode_item(g);
+  const bool live = it.col < g.DV;
   DropSeed seed{};
-  DropCol dcol{};
   if constexpr (DROP) seed = drop_seed(drop);   // whole warps
-  if (it.col >= g.DV) return;
+  if (!live && !(DROP && V == 1)) return;
   float p[4];
 #pragma unroll
   for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
   const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
-  if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
+  DropWalk<V> walk;
+  if constexpr (DROP) walk.start(seed, c0);
   using B5 = Bundle<T, V, 5>;
   auto load = [&](B5& u, int64_t s) {
+        if (!live) return;
         const T* r = Hr + (tok + s) * 4 * D + c0;
         u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
@@ -223,8 +225,11 @@ k_add_residual_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, const flo
       };
   auto compute = [&](const B5& u, int64_t s) {
         float y[V], x[V];
+        DropBits<V> bits;
+        if constexpr (DROP) bits = walk.bits(drop, tok + s, g.sub, c0);
+        if (!live) return;
         unpack<T, V>(u.p[4], y);
-        if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
+        if constexpr (DROP) drop_apply<V>(drop, bits, y);
         T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
@@ -277,14 +282,15 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
   const bool live = it.col < g.DV;
   DropSeed seed{};
   if constexpr (DROP) seed = drop_seed(drop);   // whole warps
-  if (live) {
-    DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
+  if (live || (DROP && V == 1)) {
+    DropWalk<V> walk;
+    if constexpr (DROP) walk.start(seed, c0);
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
     using B5 = Bundle<T, V, 5>;
     auto load = [&](B5& u, int64_t s) {
+      if (!live) return;
       const T* r = Hr + (tok + s) * 4 * D + c0;
       u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
@@ -292,8 +298,11 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
     };
     auto compute = [&](const B5& u, int64_t s) {
       float y[V], x[V];
+      DropBits<V> bits;
+      if constexpr (DROP) bits = walk.bits(drop, tok + s, g.sub, c0);
+      if (!live) return;
       unpack<T, V>(u.p[4], y);
-      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
+      if constexpr (DROP) drop_apply<V>(drop, bits, y);
       T* o = Hn + (tok + s) * 4 * D + c0;
 #pragma unroll
       for (int n = 0; n < 4; ++n) {
@@ -387,10 +396,10 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
   const bool live = it.col < g.DV;
   DropSeed seed{};
   if constexpr (DROP) seed = drop_seed(drop);   // whole warps
-  if (!POOL && !live) return;
-  if (live) {
-    DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
+  if (!POOL && !live && !(DROP && V == 1)) return;
+  if (live || (DROP && V == 1)) {
+    DropWalk<V> walk;
+    if constexpr (DROP) walk.start(seed, c0);
     float p[4], R[16];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
@@ -398,6 +407,7 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
     for (int k = 0; k < 16; ++k) R[k] = __ldg(Hres + it.b * 16 + k);
     using B5 = Bundle<T, V, 5>;
     auto load = [&](B5& u, int64_t s) {
+      if (!live) return;
       const T* h = H + (tok + s) * 4 * D + c0;
       u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
@@ -405,8 +415,11 @@ k_add_residual_mix_fwd(const T* __restrict__ H, const float* __restrict__ Hres, 
     };
     auto compute = [&](const B5& u, int64_t s) {
       float x[4][V], y[V], o[V];
+      DropBits<V> bits;
+      if constexpr (DROP) bits = walk.bits(drop, tok + s, g.sub, c0);
+      if (!live) return;
       unpack<T, V>(u.p[4], y);
-      if constexpr (DROP) drop_apply<V>(drop, drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0), y);
+      if constexpr (DROP) drop_apply<V>(drop, bits, y);
 #pragma unroll
       for (int n = 0; n < 4; ++n) unpack<T, V>(u.p[n], x[n]);
       T* op = Hn + (tok + s) * 4 * D + c0;
@@ -512,15 +525,17 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   DropSeed seed{};
   if constexpr (DROP) seed = drop_seed(drop);   // whole warps
-  if (it.col < g.DV) {
+  const bool live = it.col < g.DV;
+  if (live || (DROP && V == 1)) {
     float p[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) p[n] = __ldg(Hpost + it.b * 4 + n);
     const int64_t D = g.D, c0 = (int64_t)it.col * V, tok = it.b * g.S;
-    DropCol dcol{};
-    if constexpr (DROP) dcol = drop_col(seed, (uint32_t)(c0 >> 3));
+    DropWalk<V> walk;
+    if constexpr (DROP) walk.start(seed, c0);
     using B5 = Bundle<T, V, 5>;
     auto load = [&](B5& u, int64_t s) {
+          if (!live) return;
           const T* gp = G + (tok + s) * 4 * D + c0;
           u.p[4] = ld_raw<T, V>(bo + (tok + s) * D + c0);
 #pragma unroll
@@ -528,12 +543,11 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
         };
     auto compute = [&](const B5& u, int64_t s) {
           float y[V], z[V], x[V];
+          DropBits<V> bits;
+          if constexpr (DROP) bits = walk.bits(drop, tok + s, g.sub, c0);
+          if (!live) return;
           unpack<T, V>(u.p[4], y);
-          DropBits<V> bits{};
-          if constexpr (DROP) {
-            bits = drop_bits<V>(seed, dcol, drop_row(drop, seed, tok + s), c0);
-            drop_apply<V>(drop, bits, y);
-          }
+          if constexpr (DROP) drop_apply<V>(drop, bits, y);
 #pragma unroll
           for (int e = 0; e < V; ++e) z[e] = 0.f;
 #pragma unroll
@@ -1037,8 +1051,8 @@ static int add_residual_fwd_impl(const void* H_residual, const void* branch_outp
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H_residual || !branch_output || !H_post || !H_new) return fail(MHC_ERR_NULL_POINTER, "add_residual_fwd: null pointer");
   const int vec = pick_vec(dtype, D, {H_residual, branch_output, H_new});
-  const bool staged = drop && vec > 1;
-  Geo g = make_geo(S, D, vec, GeoKind::Stream, staged ? MHC_TPC_DROPFWD : MHC_TPC_ADDFWD);
+  const bool staged = drop && vec > 1;   // single columns: a block of the generator serves 8 tokens (DropWalk)
+  Geo g = make_geo(S, D, vec, GeoKind::Stream, staged ? MHC_TPC_DROPFWD : drop ? 8 : MHC_TPC_ADDFWD);
   const size_t smem = staged ? (size_t)MHC_DROP_STAGES * 5 * 16 * geo_block(g) : 0;
   g.reverse = (MHC_REV_MASK >> 2) & 1;
   const int64_t items = B * geo_slots(g);
@@ -1098,7 +1112,7 @@ static int add_residual_mix_fwd_impl(const void* H, const float* H_res, const vo
                                             geo_block(g), smem, st, (const T*)H, H_res, (const T*)branch_output, H_post,
                                             (T*)H_new, pool_partials, g, drop ? *drop : Drop{})));
   } else {
-    Geo g = make_geo(S, D, vec, GeoKind::Stream, MHC_TPC_ADDMIX);
+    Geo g = make_geo(S, D, vec, GeoKind::Stream, drop && vec == 1 ? 8 : MHC_TPC_ADDMIX);
     g.reverse = (MHC_REV_MASK >> 2) & 1;
     const int64_t items = B * geo_slots(g);
     if (int e = check_grid("add_residual_mix_fwd", items)) return e;
@@ -1175,8 +1189,8 @@ static int add_residual_bwd_impl(const void* dH_new, const void* branch_output, 
   // sizes first, pointers last: a call whose scratch is too small says so even with null pointers
   const int vec = pick_vec(dtype, D, {dH_new, branch_output, d_branch_output});
   const bool staged = drop && vec > 1;
-  Geo g = staged ? make_geo(S, D, vec, GeoKind::Reduce, drop_bwd_tpc(S, D, vec), MHC_DROP_MINB)
-                 : make_geo(S, D, vec, GeoKind::Reduce, MHC_TPC_ADDBWD, MHC_ADDBWD_OCC, MHC_FIT_COLS != 0, MHC_NARROW_MULT);
+  Geo g = drop ? make_geo(S, D, vec, GeoKind::Reduce, vec > 1 ? drop_bwd_tpc(S, D, vec) : MHC_TPC_DROPBWD, MHC_DROP_MINB)
+               : make_geo(S, D, vec, GeoKind::Reduce, MHC_TPC_ADDBWD, MHC_ADDBWD_OCC, MHC_FIT_COLS != 0, MHC_NARROW_MULT);
   const size_t smem = staged ? (size_t)MHC_DROP_STAGES * 5 * 16 * geo_block(g) : 0;
   g.reverse = (MHC_REV_MASK >> 3) & 1;
   const int64_t slots = geo_slots(g), items = B * slots;

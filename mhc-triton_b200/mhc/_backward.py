@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib as L
-from ._kernels import _check, _alpha_dev, _norm_weight, _rows
+from ._kernels import _check, _alpha_dev, _norm_weight, _rows_of
 
 _ABS0 = {"zero": L.ABS0_ZERO, "plus_one": L.ABS0_PLUS_ONE}
 _abs_grad_at_zero = "zero"
@@ -192,17 +192,17 @@ def hc_mix_backward(d_branch_input, dH_residual, dH_post, H, x, phi, H_pre_base,
 def add_residual_dropout_backward(dH_new, branch_output, H_post, rng, threshold: int, row_offset: int = 0):
     """(dH_residual, d_branch_output, dH_post [B,4] fp32) of add_residual_dropout_forward; dH_residual IS dH_new."""
     B, S, n, D = dH_new.shape
-    _check(n == 4 and tuple(branch_output.shape) == (B, S, D) and tuple(H_post.shape) == (B, 4), "shape mismatch")
-    L.require_same_device(dH_new, branch_output, H_post, rng)
+    _check(n == 4 and branch_output.shape == (B, S, D) and H_post.shape == (B, 4), "shape mismatch")
+    dev = L.same_device(dH_new, branch_output, H_post, rng)
     dH_new = dH_new.contiguous()
     branch_output = branch_output.to(dH_new.dtype).contiguous()
     H_post = L.f32c(H_post)
     d_bo = torch.empty_like(branch_output)
-    dH_post = torch.empty(B, 4, device=dH_new.device, dtype=torch.float32)
+    dH_post = torch.empty((B, 4), device=dH_new.device, dtype=torch.float32)
     buf, nbytes = L.scratch(L.OP_ADD_RESIDUAL_BWD, B, S, D, dH_new)
-    L.call_on(dH_new, "mhc_add_residual_dropout_bwd", L.ptr(dH_new), L.ptr(branch_output), L.ptr(H_post), L.ptr(rng),
-              threshold, row_offset, L.ptr(d_bo), L.ptr(dH_post), L.ptr(buf), nbytes, L.tickets(dH_new, B), B, S, D,
-              L.dtype_code(dH_new))
+    L.call_on(dev, "mhc_add_residual_dropout_bwd", dH_new.data_ptr(), branch_output.data_ptr(), H_post.data_ptr(),
+              rng.data_ptr(), threshold, row_offset, d_bo.data_ptr(), dH_post.data_ptr(), buf.data_ptr(), nbytes,
+              L.tickets(dH_new, B), B, S, D, L.dtype_code(dH_new))
     return dH_new, d_bo, dH_post
 
 
@@ -210,23 +210,25 @@ def rms_norm_backward(dy, dsum, x, residual, rstd, weight=None, rng=None, thresh
                       want_dresidual: bool = False, want_dweight: bool = True):
     """(dx, dresidual, dweight) of add_rms_norm_forward from the gradients of y and of s (dsum, or None).  Without
     dropout dresidual IS dx; dweight has the weight's type (None if not wanted)."""
-    D = x.shape[-1]
-    rows = _rows(x)
-    _check(dy.shape == x.shape and (dsum is None or dsum.shape == x.shape) and
-           (residual is None or residual.shape == x.shape) and rstd.numel() == rows, "shape mismatch")
-    L.require_same_device(x, dy, dsum, residual, rstd, weight, rng)
+    shape, dtype = x.shape, x.dtype
+    rows, D = _rows_of(x)
+    _check(dy.shape == shape and (dsum is None or dsum.shape == shape) and
+           (residual is None or residual.shape == shape) and rstd.numel() == rows, "shape mismatch")
+    dev = L.same_device(x, dy, dsum, residual, rstd, weight, rng)
     x = x.contiguous()
-    residual = None if residual is None else residual.to(x.dtype).contiguous()
-    dy = dy.to(x.dtype).contiguous()
-    dsum = None if dsum is None else dsum.to(x.dtype).contiguous()
-    w, wcode = _norm_weight(weight, x, D)
+    dy = (dy if dy.dtype == dtype else dy.to(dtype)).contiguous()
+    if residual is not None:
+        residual = (residual if residual.dtype == dtype else residual.to(dtype)).contiguous()
+    if dsum is not None:
+        dsum = (dsum if dsum.dtype == dtype else dsum.to(dtype)).contiguous()
+    w, wcode, wptr = _norm_weight(weight, dtype, D)
     dx = torch.empty_like(x)
     dres = torch.empty_like(x) if threshold and want_dresidual else None
     dw, buf, nbytes = None, None, 0
     if want_dweight and w is not None:
         dw = torch.empty_like(w)
         buf, nbytes = L.scratch(L.OP_RMS_NORM_BWD, 0, rows, D, x)
-    L.call_on(x, "mhc_rms_norm_bwd", dy.data_ptr(), L.ptr(dsum), x.data_ptr(), L.ptr(residual), rstd.data_ptr(), L.ptr(w),
+    L.call_on(dev, "mhc_rms_norm_bwd", dy.data_ptr(), L.ptr(dsum), x.data_ptr(), L.ptr(residual), rstd.data_ptr(), wptr,
               wcode, L.ptr(rng), threshold, row_offset, dx.data_ptr(), L.ptr(dres), L.ptr(dw), L.ptr(buf), nbytes, rows, D,
               L.dtype_code(x))
     if dw is not None and dw.dtype != weight.dtype:
@@ -237,19 +239,18 @@ def rms_norm_backward(dy, dsum, x, residual, rstd, weight=None, rng=None, thresh
 def stream_norm_backward(dy, H, H_pre, rstd, weight=None, want_dweight: bool = True):
     """(dH, dH_pre [B,4] fp32, dweight or None) of stream_norm_forward."""
     B, S, n, D = H.shape
-    _check(n == 4 and tuple(dy.shape) == (B, S, D) and tuple(H_pre.shape) == (B, 4) and rstd.numel() == B * S,
-           "shape mismatch")
-    L.require_same_device(H, dy, H_pre, rstd, weight)
+    _check(n == 4 and dy.shape == (B, S, D) and H_pre.shape == (B, 4) and rstd.numel() == B * S, "shape mismatch")
+    dev = L.same_device(H, dy, H_pre, rstd, weight)
     H = H.contiguous()
-    dy = dy.to(H.dtype).contiguous()
+    dy = (dy if dy.dtype == H.dtype else dy.to(H.dtype)).contiguous()
     H_pre = L.f32c(H_pre)
-    w, wcode = _norm_weight(weight, H, D)
+    w, wcode, wptr = _norm_weight(weight, H.dtype, D)
     dH = torch.empty_like(H)
-    dH_pre = torch.empty(B, 4, device=H.device, dtype=torch.float32)
+    dH_pre = torch.empty((B, 4), device=H.device, dtype=torch.float32)
     dw = torch.empty_like(w) if want_dweight and w is not None else None
     buf, nbytes = L.scratch(L.OP_STREAM_NORM_BWD, B, S, D, H)
-    L.call_on(H, "mhc_stream_norm_bwd", dy.data_ptr(), H.data_ptr(), H_pre.data_ptr(), rstd.data_ptr(), L.ptr(w), wcode,
-              dH.data_ptr(), dH_pre.data_ptr(), L.ptr(dw), L.ptr(buf), nbytes, B, S, D, L.dtype_code(H))
+    L.call_on(dev, "mhc_stream_norm_bwd", dy.data_ptr(), H.data_ptr(), H_pre.data_ptr(), rstd.data_ptr(), wptr, wcode,
+              dH.data_ptr(), dH_pre.data_ptr(), L.ptr(dw), buf.data_ptr(), nbytes, B, S, D, L.dtype_code(H))
     if dw is not None and dw.dtype != weight.dtype:
         dw = dw.to(weight.dtype)
     return dH, dH_pre, dw

@@ -216,27 +216,32 @@ def dropout_rng(rng, like: torch.Tensor) -> torch.Tensor:
         return torch.empty(2, device=like.device, dtype=torch.int64).random_()
     if torch.is_tensor(rng):
         _check(rng.dtype == torch.int64 and rng.numel() == 2, "rng must hold two int64 values (seed, offset)")
-        L.require_same_device(like, rng)
-        return rng.contiguous()
+        return rng if rng.is_contiguous() else rng.contiguous()
     seed, offset = (int(v) & 0xFFFFFFFFFFFFFFFF for v in rng)
     return torch.tensor([v - (1 << 64) if v >> 63 else v for v in (seed, offset)], device=like.device, dtype=torch.int64)
 
 
-def _rows(t: torch.Tensor) -> int:
+def _rows_of(t: torch.Tensor) -> Tuple[int, int]:
+    """(rows, columns) of a tensor whose last axis are the columns."""
+    D = t.shape[-1]
+    if D:
+        return t.numel() // D, D
     n = 1
     for s in t.shape[:-1]:
         n *= s
-    return n
+    return n, D
 
 
 def counter_dropout_forward(x: torch.Tensor, rng: torch.Tensor, threshold: int, row_offset: int = 0) -> torch.Tensor:
     """x with each element dropped (0) with probability threshold / 65536, or scaled up; rows are all axes but the last."""
-    _check(x.dim() >= 1, "x must have at least one axis")
-    L.require_same_device(x, rng)
+    if x.dim() < 1:
+        raise AssertionError("x must have at least one axis")
+    dev = L.same_device(x, rng)
     x = x.contiguous()
     y = torch.empty_like(x)
-    L.call_on(x, "mhc_counter_dropout", x.data_ptr(), rng.data_ptr(), threshold, row_offset, y.data_ptr(), _rows(x),
-              x.shape[-1], L.dtype_code(x))
+    rows, D = _rows_of(x)
+    L.call_on(dev, "mhc_counter_dropout", x.data_ptr(), rng.data_ptr(), threshold, row_offset, y.data_ptr(), rows, D,
+              L.dtype_code(x))
     return y
 
 
@@ -246,9 +251,9 @@ def add_residual_dropout_forward(H, H_res, branch_output, H_post, rng, threshold
     branch_output passed through the counter-based dropout."""
     _check(H.dim() == 4 and H.shape[2] == 4, "H must be [batch, seq, 4, dim]")
     B, S, _, D = H.shape
-    _check(tuple(branch_output.shape) == (B, S, D), "branch_output shape mismatch")
-    _check(tuple(H_post.shape) == (B, 4) and (H_res is None or tuple(H_res.shape) == (B, 4, 4)), "weight shape mismatch")
-    L.require_same_device(H, H_res, branch_output, H_post, rng)
+    _check(branch_output.shape == (B, S, D), "branch_output shape mismatch")
+    _check(H_post.shape == (B, 4) and (H_res is None or H_res.shape == (B, 4, 4)), "weight shape mismatch")
+    dev = L.same_device(H, H_res, branch_output, H_post, rng)
     H = H.contiguous()
     branch_output = branch_output.to(H.dtype).contiguous()
     H_post = L.f32c(H_post)
@@ -258,8 +263,8 @@ def add_residual_dropout_forward(H, H_res, branch_output, H_post, rng, threshold
     if pool:
         chunks = L.load().mhc_add_residual_pool_chunks(S, D)
         partials = torch.empty(B, chunks, 4 * D, device=H.device, dtype=torch.float32)
-    L.call_on(H, "mhc_add_residual_dropout_fwd", L.ptr(H), L.ptr(H_res), L.ptr(branch_output), L.ptr(H_post), L.ptr(rng),
-              threshold, row_offset, L.ptr(H_new), L.ptr(partials), B, S, D, L.dtype_code(H))
+    L.call_on(dev, "mhc_add_residual_dropout_fwd", H.data_ptr(), L.ptr(H_res), branch_output.data_ptr(), H_post.data_ptr(),
+              rng.data_ptr(), threshold, row_offset, H_new.data_ptr(), L.ptr(partials), B, S, D, L.dtype_code(H))
     return (H_new, partials) if pool else H_new
 
 
@@ -268,37 +273,41 @@ _E4M3 = torch.float8_e4m3fn
 _SCALES = {torch.float32: L.SCALE_F32, torch.float8_e8m0fnu: L.SCALE_E8M0}
 
 
-def _norm_weight(weight, x, D) -> Tuple[Optional[torch.Tensor], int]:
-    """The weight as the kernels take it (fp32 or x's type, contiguous) and its type code."""
+def _norm_weight(weight, dtype, D) -> Tuple[Optional[torch.Tensor], int, Optional[int]]:
+    """The weight as the kernels take it (fp32 or the activations' type, contiguous), its type code and its address."""
     if weight is None:
-        return None, L.MHC_F32
-    _check(tuple(weight.shape) == (D,), f"weight shape mismatch: {tuple(weight.shape)} vs ({D},)")
-    if weight.dtype != x.dtype and weight.dtype != torch.float32:
+        return None, L.MHC_F32, None
+    if weight.shape != (D,):
+        raise AssertionError(f"weight shape mismatch: {tuple(weight.shape)} vs ({D},)")
+    if weight.dtype != dtype and weight.dtype != torch.float32:
         weight = weight.float()
-    return weight.contiguous(), L.dtype_code(weight)
+    weight = weight.contiguous()
+    return weight, L.dtype_code(weight), weight.data_ptr()
 
 
-def _norm_inputs(x, residual, weight, rng=None):
-    _check(x.dim() >= 1, "x must have at least one axis")
-    L.require_same_device(x, residual, weight, rng)
+def _norm_inputs(x, residual):
+    if x.dim() < 1:
+        raise AssertionError("x must have at least one axis")
     if residual is not None:
-        _check(residual.shape == x.shape, f"residual shape mismatch: {tuple(residual.shape)} vs {tuple(x.shape)}")
-        residual = residual.to(x.dtype).contiguous()
+        if residual.shape != x.shape:
+            raise AssertionError(f"residual shape mismatch: {tuple(residual.shape)} vs {tuple(x.shape)}")
+        residual = (residual if residual.dtype == x.dtype else residual.to(x.dtype)).contiguous()
     return x.contiguous(), residual
 
 
 def add_rms_norm_forward(x, residual=None, weight=None, eps: float = 1e-6, rng=None, threshold: int = 0,
                          row_offset: int = 0, want_rstd: bool = True):
     """(y, s, rstd): s = dropout(x) + residual (x itself when there is neither), y = s * rstd * weight."""
-    x, residual = _norm_inputs(x, residual, weight, rng)
-    D = x.shape[-1]
-    w, wcode = _norm_weight(weight, x, D)
+    dev = L.same_device(x, residual, weight, rng)
+    x, residual = _norm_inputs(x, residual)
+    rows, D = _rows_of(x)
+    w, wcode, wptr = _norm_weight(weight, x.dtype, D)
     y = torch.empty_like(x)
     s = torch.empty_like(x) if residual is not None or threshold else None
-    rows = _rows(x)
     rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
-    L.call_on(x, "mhc_add_rms_norm_fwd", x.data_ptr(), L.ptr(residual), L.ptr(w), wcode, L.ptr(rng), threshold, row_offset,
-              L.ptr(s), y.data_ptr(), L.ptr(rstd), rows, D, L.dtype_code(x), eps)
+    L.call_on(dev, "mhc_add_rms_norm_fwd", x.data_ptr(), None if residual is None else residual.data_ptr(), wptr, wcode,
+              L.ptr(rng), threshold, row_offset, None if s is None else s.data_ptr(), y.data_ptr(), L.ptr(rstd), rows, D,
+              L.dtype_code(x), eps)
     return y, (x if s is None else s), rstd
 
 
@@ -309,54 +318,54 @@ def _scales_for(lead, D, group, scale_dtype, device):
     if scale_dtype not in _SCALES:
         raise TypeError(f"mhc: unsupported scale dtype {scale_dtype} (float32, float8_e8m0fnu only)")
     G = -(-D // group) if group else 1
-    return group, _SCALES[scale_dtype], torch.empty(*lead, G, device=device, dtype=scale_dtype)
+    return group, _SCALES[scale_dtype], torch.empty((*lead, G), device=device, dtype=scale_dtype)
 
 
 def add_rms_norm_quant_forward(x, residual=None, weight=None, eps: float = 1e-6, group=None,
                                scale_dtype=torch.float32):
     """(q, scales, s): the norm's output as e4m3 q with one scale per row or per `group` columns."""
-    x, residual = _norm_inputs(x, residual, weight)
-    D = x.shape[-1]
-    w, wcode = _norm_weight(weight, x, D)
+    dev = L.same_device(x, residual, weight)
+    x, residual = _norm_inputs(x, residual)
+    rows, D = _rows_of(x)
+    w, wcode, wptr = _norm_weight(weight, x.dtype, D)
     group, scode, scales = _scales_for(x.shape[:-1], D, group, scale_dtype, x.device)
-    q = torch.empty(x.shape, device=x.device, dtype=_E4M3)
+    q = torch.empty_like(x, dtype=_E4M3)
     s = torch.empty_like(x) if residual is not None else None
-    L.call_on(x, "mhc_add_rms_norm_quant_fwd", x.data_ptr(), L.ptr(residual), L.ptr(w), wcode, L.ptr(s), q.data_ptr(),
-              scales.data_ptr(), group, scode, _rows(x), D, L.dtype_code(x), eps)
+    L.call_on(dev, "mhc_add_rms_norm_quant_fwd", x.data_ptr(), L.ptr(residual), wptr, wcode, L.ptr(s), q.data_ptr(),
+              scales.data_ptr(), group, scode, rows, D, L.dtype_code(x), eps)
     return q, scales, (x if s is None else s)
 
 
 def _stream_inputs(H, H_pre, weight):
-    _check(H.dim() == 4 and H.shape[2] == 4, "H must be [batch, seq, 4, dim]")
-    B, S, _, D = H.shape
-    _check(tuple(H_pre.shape) == (B, 4), f"H_pre shape mismatch: {tuple(H_pre.shape)} vs ({B}, 4)")
-    L.require_same_device(H, H_pre, weight)
-    H = H.contiguous()
-    w, wcode = _norm_weight(weight, H, D)
-    return H, L.f32c(H_pre), w, wcode
+    if H.dim() != 4 or H.shape[2] != 4:
+        raise AssertionError("H must be [batch, seq, 4, dim]")
+    if H_pre.shape != (H.shape[0], 4):
+        raise AssertionError(f"H_pre shape mismatch: {tuple(H_pre.shape)} vs ({H.shape[0]}, 4)")
+    dev = L.same_device(H, H_pre, weight)
+    return dev, H.contiguous(), L.f32c(H_pre), _norm_weight(weight, H.dtype, H.shape[3])
 
 
 def stream_norm_forward(H, H_pre, weight=None, eps: float = 1e-6, want_branch_input: bool = False,
                         want_rstd: bool = True):
     """(y, branch_input or None, rstd [B*S]): branch_input = sum_n H_pre[n] H[n], y its norm times weight."""
-    H, H_pre, w, wcode = _stream_inputs(H, H_pre, weight)
+    dev, H, H_pre, (w, wcode, wptr) = _stream_inputs(H, H_pre, weight)
     B, S, _, D = H.shape
-    y = torch.empty(B, S, D, device=H.device, dtype=H.dtype)
+    y = torch.empty((B, S, D), device=H.device, dtype=H.dtype)
     bi = torch.empty_like(y) if want_branch_input else None
     rstd = torch.empty(B * S, device=H.device, dtype=torch.float32) if want_rstd else None
-    L.call_on(H, "mhc_stream_norm_fwd", H.data_ptr(), H_pre.data_ptr(), L.ptr(w), wcode, L.ptr(bi), y.data_ptr(),
-              L.ptr(rstd), B, S, D, L.dtype_code(H), eps)
+    L.call_on(dev, "mhc_stream_norm_fwd", H.data_ptr(), H_pre.data_ptr(), wptr, wcode, L.ptr(bi), y.data_ptr(), L.ptr(rstd),
+              B, S, D, L.dtype_code(H), eps)
     return y, bi, rstd
 
 
 def stream_norm_quant_forward(H, H_pre, weight=None, eps: float = 1e-6, group=None, scale_dtype=torch.float32):
     """(q, scales): stream_norm_forward's y as e4m3 with one scale per token or per `group` columns."""
-    H, H_pre, w, wcode = _stream_inputs(H, H_pre, weight)
+    dev, H, H_pre, (w, wcode, wptr) = _stream_inputs(H, H_pre, weight)
     B, S, _, D = H.shape
     group, scode, scales = _scales_for((B, S), D, group, scale_dtype, H.device)
-    q = torch.empty(B, S, D, device=H.device, dtype=_E4M3)
-    L.call_on(H, "mhc_stream_norm_quant_fwd", H.data_ptr(), H_pre.data_ptr(), L.ptr(w), wcode, q.data_ptr(),
-              scales.data_ptr(), group, scode, B, S, D, L.dtype_code(H), eps)
+    q = torch.empty((B, S, D), device=H.device, dtype=_E4M3)
+    L.call_on(dev, "mhc_stream_norm_quant_fwd", H.data_ptr(), H_pre.data_ptr(), wptr, wcode, q.data_ptr(), scales.data_ptr(),
+              group, scode, B, S, D, L.dtype_code(H), eps)
     return q, scales
 
 
@@ -369,9 +378,9 @@ def hc_mix_norm_forward(H, H_pre_base, H_post_base, H_res_base, phi, alpha_pre, 
     _check(S > 0 and D > 0, "empty sequence or width")
     _check(tuple(phi.shape) == (4 * D, 24), f"phi shape mismatch: {tuple(phi.shape)} vs ({4 * D}, 24)")
     _check(H_pre_base.numel() == 4 and H_post_base.numel() == 4 and H_res_base.numel() == 16, "base parameter shapes")
-    L.require_same_device(H, phi, H_pre_base, H_post_base, H_res_base, norm_weight)
+    index = L.same_device(H, phi, H_pre_base, H_post_base, H_res_base, norm_weight)
     H = H.contiguous()
-    w, wcode = _norm_weight(norm_weight, H, D)
+    w, wcode, wptr = _norm_weight(norm_weight, H.dtype, D)
     phi, pre_b, post_b, res_b = L.f32c(phi), L.f32c(H_pre_base), L.f32c(H_post_base), L.f32c(H_res_base)
     a = [_alpha_dev(v, H) for v in (alpha_pre, alpha_post, alpha_res)]
     dev = H.device
@@ -388,8 +397,8 @@ def hc_mix_norm_forward(H, H_pre_base, H_post_base, H_res_base, phi, alpha_pre, 
         _check(pooled.dim() == 3 and pooled.shape[0] == B and pooled.shape[2] == 4 * D and pooled.dtype == torch.float32
                and pooled.is_contiguous() and pooled.device == dev, "pooled must be contiguous fp32 [B, chunks, 4*D]")
         chunks = pooled.shape[1]
-    L.call_on(H, "mhc_hc_mix_norm_fwd", L.ptr(H), L.ptr(phi), L.ptr(pre_b), L.ptr(post_b), L.ptr(res_b), L.ptr(a[0]),
-              L.ptr(a[1]), L.ptr(a[2]), L.ptr(w), wcode, float(norm_eps), L.ptr(x), L.ptr(H_pre), L.ptr(H_post),
+    L.call_on(index, "mhc_hc_mix_norm_fwd", L.ptr(H), L.ptr(phi), L.ptr(pre_b), L.ptr(post_b), L.ptr(res_b), L.ptr(a[0]),
+              L.ptr(a[1]), L.ptr(a[2]), wptr, wcode, float(norm_eps), L.ptr(x), L.ptr(H_pre), L.ptr(H_post),
               L.ptr(H_res), L.ptr(saved), L.ptr(bi), L.ptr(y), L.ptr(rstd), L.ptr(pooled), chunks, L.ptr(buf), nbytes,
               L.tickets(H, B), B, S, D, L.dtype_code(H), int(sinkhorn_iters), float(eps))
     return y, bi, rstd, H_post, H_pre, H_res, x, saved

@@ -5,6 +5,7 @@ device, the call raises.  Build the library with ``python mhc-triton_b200/build.
 """
 
 import ctypes
+import functools
 import os
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
@@ -112,14 +113,16 @@ def call(name, stream, *args):
     return check(getattr(load(), name)(*args, stream))
 
 
-def call_on(like: torch.Tensor, name, *args):
-    """Invoke an entry point on torch's current stream of `like`'s device, with that device current."""
-    dev = like.device
-    stream = torch._C._cuda_getCurrentRawStream(dev.index)
-    if dev.index == torch.cuda.current_device():
-        return check(getattr(_lib or load(), name)(*args, stream))
-    with torch.cuda.device(dev):
-        return check(getattr(_lib or load(), name)(*args, stream))
+def call_on(dev: int, name, *args):
+    """Invoke an entry point on torch's current stream of device `dev`, with that device current."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch._C._cuda_getDevice():
+        status = getattr(_lib or load(), name)(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            status = getattr(_lib or load(), name)(*args, stream)
+    if status:
+        check(status)
 
 
 def profile_start(only=None):
@@ -162,13 +165,15 @@ def require_cuda(*tensors):
             raise RuntimeError("mhc: tensors must live on a CUDA device (this build has no CPU path)")
 
 
-def require_same_device(like, *tensors):
-    """`like` and every tensor given (None is skipped) on one CUDA device."""
-    if not like.is_cuda:
+def same_device(like, *tensors) -> int:
+    """The CUDA device index that `like` and every tensor given (None is skipped) live on."""
+    dev = like.get_device()
+    if dev < 0:
         raise RuntimeError("mhc: tensors must live on a CUDA device (this build has no CPU path)")
     for t in tensors:
-        if t is not None and t.device != like.device:
+        if t is not None and t.get_device() != dev:
             raise RuntimeError(f"mhc: tensors must live on one CUDA device, got {like.device} and {t.device}")
+    return dev
 
 
 def ptr(t):
@@ -181,11 +186,17 @@ def stream_of(t: torch.Tensor):
                                               else torch.cuda.current_device())
 
 
-def scratch(op, B, S, D, like: torch.Tensor):
-    """Caller-owned scratch for `op`, taken from torch's caching allocator."""
-    n = load().mhc_scratch_bytes(op, B, S, D, _DTYPE_CODE.get(like.dtype, MHC_F32))
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(op, B, S, D, dtype):
+    n = load().mhc_scratch_bytes(op, B, S, D, dtype)
     if n < 0:
         raise MhcError("mhc_scratch_bytes: bad arguments")
+    return n
+
+
+def scratch(op, B, S, D, like: torch.Tensor):
+    """Caller-owned scratch for `op`, taken from torch's caching allocator."""
+    n = _scratch_bytes(op, B, S, D, _DTYPE_CODE.get(like.dtype, MHC_F32))
     return torch.empty(max(n, 4) // 4, device=like.device, dtype=torch.float32), n
 
 

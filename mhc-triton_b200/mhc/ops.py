@@ -256,6 +256,13 @@ class _AddResidualDropout(torch.autograd.Function):
         return (dH_residual, None, None, d_bo.to(branch_output.dtype), dH_post.to(H_post.dtype)) + (None,) * 4
 
 
+def _first_order(backward):
+    """once_differentiable (an error where a gradient's gradient is asked for) at no cost where none can be: grad mode
+    is on in a backward only with create_graph=True."""
+    checked = once_differentiable(backward)
+    return lambda ctx, *grads: checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _CounterDropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rng, threshold, row_offset):
@@ -264,7 +271,7 @@ class _CounterDropout(torch.autograd.Function):
         return counter_dropout_forward(x, rng, threshold, row_offset)
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad):
         (rng,) = ctx.saved_tensors
         return counter_dropout_forward(grad, rng, ctx.threshold, ctx.row_offset), None, None, None
@@ -282,7 +289,7 @@ class _AddRmsNorm(torch.autograd.Function):
         return (y, s) if residual is not None or threshold else y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy, ds=None):
         if dy is None and ds is None:
             return (None,) * 7
@@ -292,7 +299,9 @@ class _AddRmsNorm(torch.autograd.Function):
         need_x, need_res, need_w = ctx.needs_input_grad[:3]
         dx, dres, dw = rms_norm_backward(dy, ds, x, residual, rstd, weight, rng, ctx.threshold, ctx.row_offset,
                                          want_dresidual=need_res, want_dweight=need_w)
-        return (dx if need_x else None, dres.to(residual.dtype) if need_res else None, dw, None, None, None, None)
+        if need_res and dres.dtype != residual.dtype:
+            dres = dres.to(residual.dtype)
+        return dx if need_x else None, dres if need_res else None, dw, None, None, None, None
 
 
 class _FusedStreamNorm(torch.autograd.Function):
@@ -303,11 +312,11 @@ class _FusedStreamNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, dy):
         H, H_pre, weight, rstd = ctx.saved_tensors
         dH, dH_pre, dw = stream_norm_backward(dy, H, H_pre, rstd, weight, want_dweight=ctx.needs_input_grad[2])
-        return dH, dH_pre.to(H_pre.dtype), dw, None
+        return dH, (dH_pre if dH_pre.dtype == H_pre.dtype else dH_pre.to(H_pre.dtype)), dw, None
 
 
 @torch.compiler.disable
@@ -432,7 +441,12 @@ def hyper_connection_mix(H, H_pre_base, H_post_base, H_res_base, phi, alpha_pre,
 
 
 def _records(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether autograd would record an operation on these."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 @torch.compiler.disable

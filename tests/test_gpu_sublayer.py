@@ -47,7 +47,7 @@ def subnormal(dtype):
 
 # rows, columns: one token, one column, below and over a pack, a warp, a CTA; odd widths; widths of the layer stacks; many rows
 SHAPES = [(1, 1), (3, 7), (1, 4096), (2, 8), (5, 64), (37, 129), (1000, 96), (17, 1000), (9, 1021), (6, 2048), (700, 512),
-          (4, 7168), (3, 8200), (2, 16384), (2, 12289), (2, 40000)]
+          (4, 7168), (3, 8200), (2, 16384), (2, 12289), (2, 40000), (1500, 584), (3000, 40), (5, 8191), (3, 8193), (650, 279), (700, 3000)]
 
 
 def norm_case(rows, D, dtype, wdtype, residual, seed=0, p=0.0, zero_row=True):
@@ -125,6 +125,31 @@ def test_add_rms_norm(rows, D, dt, wdt, residual, p):
         within(grads["w"], dw64, hw * dw64.abs() + (rows_chain + steps(D)) * U * dw_mag * s_rel.max() + subnormal(w.dtype), "dw")
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("lo", range(0, 4608, 512))
+def test_add_rms_norm_every_kind_of_width(dt, lo):
+    """Widths that change the threads per row, the rows per block and the last pack, against 64 bits."""
+    import mhc
+    dtype = TYPES[dt]
+    h = half_step(dtype)
+    for D in [lo + d for d in (4, 8, 31, 72, 120, 256, 264, 391, 392, 504)]:
+        rows = 700 if D < 1024 else 300
+        x, r, w = norm_case(rows, D, dtype, torch.float32, True, seed=D, zero_row=False)
+        dy, ds = draw((rows, D), dtype, D + 1), draw((rows, D), dtype, D + 2)
+        leaves = [t.cuda().requires_grad_(True) for t in (x, r, w)]
+        y, s = mhc.fused_add_rms_norm(*leaves, EPS)
+        grads = torch.autograd.grad([y, s], leaves, [dy.cuda(), ds.cuda()])
+        s64 = x.double() + r.double()
+        y64, rstd = SO.rms_norm(s64, w.double(), EPS)
+        k = steps(D) * U
+        within(y, y64, (h + 2 * k) * y64.abs() + 1e-30, f"y {D}")
+        g64, dw64, g_mag, dw_mag = SO.rms_norm_grad(dy.double(), s64, rstd, w.double())
+        g64, g_mag = g64 + ds.double(), g_mag + ds.double().abs()
+        for got in grads[:2]:
+            within(got, g64, h * g64.abs() + 2 * k * g_mag + 1e-30, f"dx {D}")
+        within(grads[2], dw64, (rows + 40 + steps(D)) * U * dw_mag, f"dw {D}")
+
+
 def check_quant(q, scales, y64, y_err, group, e8m0, D):
     """q, scales against fp64 y whose fp32 counterpart is off by at most y_err (elementwise)."""
     G = -(-D // group) if group else 1
@@ -180,7 +205,7 @@ def stream_case(B, S, D, dtype, seed):
 
 
 STREAM_SHAPES = [(1, 1, 8), (2, 3, 64), (3, 5, 33), (1, 130, 256), (5, 1, 4096), (2, 19, 1000), (1, 3, 1021), (2, 2, 7168),
-                 (300, 2, 40), (1, 2, 16384), (1, 2, 33000), (2, 700, 512)]
+                 (300, 2, 40), (1, 2, 16384), (1, 2, 33000), (2, 700, 512), (2, 333, 584), (1, 301, 999), (3, 40, 2049)]
 
 
 def mixed64(H, pre):
