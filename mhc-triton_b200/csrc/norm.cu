@@ -35,11 +35,12 @@ struct NormFwd {
   void* scales;          // [rows, G] fp32 or e8m0 bytes
   float* rstd;           // [rows] or null
   int64_t rows, S, D;
-  int group;             // columns per scale (GroupScale)
+  int group, shift;      // columns per scale (GroupScale): 1 << shift
+  int G;                 // scales per row
   int e8m0;
   float eps;
   float inv_D;
-  double inv_D64;
+  float inv_D_lo;        // 1 / D = inv_D + inv_D_lo
   Drop drop;
 };
 
@@ -59,7 +60,6 @@ struct NormBwd {
   int64_t items, S, D;   // items: rows (Add), batch elements x chunks (Mix)
   int parts;             // rows of dw_part
   int64_t chunks;        // per batch element (Mix)
-  int tpc;               // tokens per chunk (Mix)
   float inv_D;
   Drop drop;
 };
@@ -82,24 +82,46 @@ __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return r;
 }
 
+// 1 / sqrt(mean + eps) from a sum of squares: the hardware's approximation (2^-22.9) and one Newton step.
+__device__ __forceinline__ float row_rstd(float ss, float inv_D, float eps) {
+  const float x = fmaf(ss, inv_D, eps), r = rsqrtf(x);
+  return x > 1e-30f && x < 1e30f ? fmaf(0.5f * r, fmaf(-x * r, r, 1.f), r) : r;   // elsewhere the step itself would lose
+}
+// The same to about 45 bits, as hi + lo, for 8-bit outputs, where an error of the last fp32 bit moves a value or a
+// power-of-two scale that is next to a border to the other side (1 scale in 4 million at 16384 x 7168).  Products and
+// their exact errors by FMA; in fp64 it cost 9 us of 133 at that shape.
+struct Rstd2 { float hi, lo; };
+__device__ __forceinline__ Rstd2 row_rstd2(float ss, float inv_hi, float inv_lo, float eps) {
+  const float p = ss * inv_hi, pe = fmaf(ss, inv_hi, -p) + ss * inv_lo;   // mean = p + pe
+  const float x = p + eps, big = fmaxf(p, eps), small = fminf(p, eps);
+  const float xe = (big - x + small) + pe;                                // x + xe = mean + eps
+  Rstd2 r;
+  r.hi = rsqrtf(x);
+  const float t = x * r.hi, te = fmaf(x, r.hi, -t) + xe * r.hi;           // (x + xe) hi
+  const float e = fmaf(-t, r.hi, 1.f) - te * r.hi;                        // 1 - (x + xe) hi^2
+  r.lo = x > 1e-30f && x < 1e30f ? 0.5f * r.hi * e : 0.f;
+  return r;
+}
+
 // Scale of the values u rstd whose largest |u| is `umax`, and the two factors that take u itself to e4m3.
 // fp32: scale = umax rstd / 448 and u (448 / umax): rstd cancels, so a quotient is two roundings from s w.
 // e8m0: the next power of two that is not below the largest |value| / 448 (so nothing saturates), as its biased
 // exponent: 448 = 1.75 * 2^8, so that is the value's exponent - 8, plus one if its mantissa is above 1.75, which the
 // carry of an integer addition says exactly; NaN and infinity become the NaN code 255.
 struct Scale { float f1, f2, f32; uint32_t code; };
-__device__ __forceinline__ Scale make_scale(float umax, double rstd, int e8m0) {
+__device__ __forceinline__ Scale make_scale(float umax, const Rstd2& rstd, int e8m0) {
   Scale r;
-  r.f1 = (float)rstd;
+  r.f1 = rstd.hi + rstd.lo;
+  const float amax = fmaf(umax, rstd.hi, umax * rstd.lo);
   if (e8m0) {
-    const uint32_t b = __float_as_uint((float)((double)umax * rstd));
+    const uint32_t b = __float_as_uint(amax);
     const int e = (int)((b + 0x1fffffu) >> 23) - 8;
     const bool finite = b < 0x7f800000u;
     r.code = finite ? (uint32_t)(e < 1 ? 1 : e) : 255u;
     r.f32 = 0.f;   // not stored
     r.f2 = finite ? __uint_as_float((254u - r.code) << 23) : __int_as_float(0x7fc00000);
   } else {
-    const float s = (float)((double)umax * rstd * (1.0 / kE4m3Max));
+    const float s = __fdiv_rn(amax, kE4m3Max);
     r.code = 0;
     if (s < kMinScale) {  // false for NaN
       r.f32 = kMinScale;
@@ -113,19 +135,6 @@ __device__ __forceinline__ Scale make_scale(float umax, double rstd, int e8m0) {
   return r;
 }
 
-// 1 / sqrt(mean + eps) from a sum of squares: the hardware's approximation (2^-22.9) and one Newton step.
-__device__ __forceinline__ float row_rstd(float ss, float inv_D, float eps) {
-  const float x = fmaf(ss, inv_D, eps), r = rsqrtf(x);
-  return x > 1e-30f && x < 1e30f ? fmaf(0.5f * r, fmaf(-x * r, r, 1.f), r) : r;   // elsewhere the step itself would lose
-}
-// The same in fp64 for 8-bit outputs, where an error of the last fp32 bit moves a value or a power-of-two scale that is
-// next to a border to the other side (1 scale in 4 million at 16384 x 7168): five fp64 operations per thread and row.
-__device__ __forceinline__ double row_rstd64(float ss, double inv_D, float eps) {
-  const double x = (double)ss * inv_D + (double)eps;
-  const float f = rsqrtf((float)x);
-  const double r = (double)f;
-  return f > 1e-15f && f < 1e15f ? r + 0.5 * r * (1.0 - x * r * r) : r;
-}
 __device__ __forceinline__ void store_scale(void* scales, int64_t i, const Scale& s, int e8m0) {
   if (e8m0) ((uint8_t*)scales)[i] = (uint8_t)s.code;
   else ((float*)scales)[i] = s.f32;
@@ -200,15 +209,15 @@ k_norm_any_fwd(NormFwd a) {
       ((T*)a.y)[row * D + d] =
           from_f32<T>(src_at<T, SRC, DROP>(a, seed, pre, row, d) * rstd * load_w<T>(a.weight, a.w_f32, d));
   } else if constexpr (OUT == Out::RowScale) {
-    const Scale s = make_scale(mx, row_rstd64(ss, a.inv_D64, a.eps), a.e8m0);
+    const Scale s = make_scale(mx, row_rstd2(ss, a.inv_D, a.inv_D_lo, a.eps), a.e8m0);
     if (threadIdx.x == 0) store_scale(a.scales, row, s, a.e8m0);
     for (int64_t d = threadIdx.x; d < D; d += 256) {
       const float u = src_at<T, SRC, DROP>(a, seed, pre, row, d) * load_w<T>(a.weight, a.w_f32, d);
       ((uint8_t*)a.y)[row * D + d] = (uint8_t)e4m3x2(u * s.f1 * s.f2, 0.f);
     }
   } else {  // a warp per group
-    const double rstd = row_rstd64(ss, a.inv_D64, a.eps);
-    const int64_t G = (D + a.group - 1) / a.group;
+    const Rstd2 rstd = row_rstd2(ss, a.inv_D, a.inv_D_lo, a.eps);
+    const int64_t G = a.G;
     const int lane = threadIdx.x & 31;
     for (int64_t g = threadIdx.x >> 5; g < G; g += 8) {
       float y[4], m = 0.f;
@@ -251,13 +260,13 @@ k_norm_any_bwd(NormBwd a) {
     int64_t r0 = it, r1 = it + 1;   // RowMap of this kernel: one row at a time
     float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (SRC == Src::Mix) {
-      const int64_t b = it / a.chunks, c = it % a.chunks;
-      r0 = b * a.S + c * a.tpc;
-      r1 = min(r0 + a.tpc, (b + 1) * a.S);
+      const int64_t b = it / a.chunks;
+      r0 = b * a.S + it % a.chunks;
+      r1 = (b + 1) * a.S;
 #pragma unroll
       for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + b * 4 + n);
     }
-    for (int64_t row = r0; row < r1; ++row) {
+    for (int64_t row = r0; row < r1; row += SRC == Src::Mix ? a.chunks : 1) {
       const float rstd = __ldg(a.rstd + row);
       NormFwd f;
       f.x = a.x; f.res = a.res; f.sum_out = nullptr; f.D = D; f.drop = a.drop;
@@ -431,7 +440,7 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
       if (pk.first + k * pk.step < DV) PackIO<T, V>::store((T*)a.y + at + k * stride, v[k]);
     }
   } else {
-    const double rstd = row_rstd64(ss, a.inv_D64, a.eps);
+    const Rstd2 rstd = row_rstd2(ss, a.inv_D, a.inv_D_lo, a.eps);
     Scale sc{};
     float g[NP];   // largest |v w| of the group a pack is in
     if constexpr (OUT == Out::RowScale) {
@@ -447,8 +456,6 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
         if (OUT == Out::GroupScale) g[k] = max_nan(g[k], fabsf(v[k][e]));
       }
     }
-    const int lanes = V > 1 ? a.group / V : 32;   // consecutive lanes that share a group
-    const int G = OUT == Out::GroupScale ? ((int)a.D + a.group - 1) / a.group : 1;
     if constexpr (OUT == Out::GroupScale && V == 1) {   // 64 or 128 columns are 2 or 4 consecutive k of the warp
 #pragma unroll
       for (int k = 0; k < NP; k += 2)
@@ -461,10 +468,12 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
     for (int k = 0; k < NP; ++k) {
       const int p = pk.first + k * pk.step;
       if constexpr (OUT == Out::GroupScale) {
-        for (int o = lanes >> 1; o > 0; o >>= 1) g[k] = max_nan(g[k], __shfl_xor_sync(0xffffffffu, g[k], o));
+        // group / V consecutive lanes share it (V = 1: the warp)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+          if (V == 1 || o * V < 32 || o * V < a.group) g[k] = max_nan(g[k], __shfl_xor_sync(0xffffffffu, g[k], o));
         sc = make_scale(g[k], rstd, a.e8m0);
-        if (p < DV && (p * V & (a.group - 1)) == 0)
-          store_scale(a.scales, row * G + (uint32_t)(p * V) / (uint32_t)a.group, sc, a.e8m0);
+        if (p < DV && (p * V & (a.group - 1)) == 0) store_scale(a.scales, row * a.G + (p * V >> a.shift), sc, a.e8m0);
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] *= sc.f1;
@@ -670,8 +679,8 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
 // Backward: persistent CTAs, so that the threads, which own the same columns in every row, keep the weight and
 // dweight's running sums in registers.  The packs of the next DEPTH - 1 rows are on the way meanwhile, by cp.async into
 // slots of shared memory that only the thread itself reads (no barrier): in registers they spilled, and the
-// stream form ran at 42 % of the memory's rate.  An item is rpc rows (Add) or a chunk of a batch element's tokens
-// (Mix), walked rpc abreast.  DEPTH 0 (single elements, which cp.async cannot copy): loads straight from memory.
+// stream form ran at 42 % of the memory's rate.  An item is rpc rows (Add) or one of `chunks` shares of a batch element's
+// tokens (Mix): every chunks-th group of rpc tokens, so that the CTAs sweep the memory side by side.  DEPTH 0 (single elements, which cp.async cannot copy): loads straight from memory.
 template <typename T, int V, int NP, int DEPTH, int THREADS, Src SRC, bool DROP>
 __global__ void __launch_bounds__(THREADS)
 k_norm_bwd(NormBwd a, RowMap m) {
@@ -703,16 +712,16 @@ k_norm_bwd(NormBwd a, RowMap m) {
     if (q.item >= a.items) return;
     if constexpr (SRC == Src::Mix) {
       const int64_t b = q.item / a.chunks, c = q.item - b * a.chunks;
-      q.base = b * a.S + c * a.tpc;
-      q.end = min(q.base + a.tpc, (b + 1) * a.S);
+      q.base = b * a.S + c * m.rpc;
+      q.end = (b + 1) * a.S;
     } else {
       q.base = q.item * m.rpc;
       q.end = min(q.base + m.rpc, a.S);
     }
   };
   auto next = [&](Pos q) -> Pos {
-    q.base += m.rpc;
-    if (q.base >= q.end) {
+    q.base += SRC == Src::Mix ? a.chunks * m.rpc : m.rpc;
+    if (SRC == Src::Add || q.base >= q.end) {
       q.item += gridDim.x;
       enter(q);
     }
@@ -955,15 +964,13 @@ static int64_t bwd_ctas(int64_t items, int threads) {
   const int64_t most = (threads > 256 ? 1 : 2) * (int64_t)sm_count();
   return items < most ? items : most;
 }
-// Tokens per chunk of the stream-norm backward: as many chunks per batch element as fill the device's CTAs once (so any
-// number of batch elements fills them evenly), but four rounds of rpc tokens at least, since a chunk ends with a
+// Shares that the stream-norm backward divides a batch element's tokens into: as many as fill the device's CTAs once (so any
+// number of batch elements fills them evenly), but four rounds of rpc tokens each at least, since a share ends with a
 // reduction.  A function of the sequence and the width only: a batch element sums in the same order in any batch.
-static int64_t mix_tpc(int64_t S, int rpc) {
-  const int64_t even = (S + 2 * sm_count() - 1) / (2 * sm_count()), least = S < 4 * rpc ? S : 4 * rpc;
-  const int64_t n = even > least ? even : least;
-  return n > 0 ? n : 1;
+static int64_t mix_chunks(int64_t S, int rpc) {
+  const int64_t groups = (S + rpc - 1) / rpc, most = 2 * (int64_t)sm_count(), few = (groups + 3) / 4;
+  return groups <= 4 ? (groups > 0 ? 1 : 0) : few < most ? few : most;
 }
-static int64_t mix_chunks(int64_t S, int rpc) { return (S + mix_tpc(S, rpc) - 1) / mix_tpc(S, rpc); }
 
 #ifndef MHC_RING_MIN
 #define MHC_RING_MIN 4
@@ -1026,6 +1033,18 @@ static int check_quant(const char* what, int64_t group, int scale_type) {
   return MHC_OK;
 }
 
+static void set_group(NormFwd& a, int64_t group, int64_t D) {
+  a.group = (int)group;
+  a.shift = group == 32 ? 5 : group == 64 ? 6 : 7;
+  a.G = group ? (int)((D + group - 1) / group) : 1;
+}
+
+static void set_inv(NormFwd& a, int64_t D) {
+  const double inv = 1.0 / (double)D;
+  a.inv_D = (float)inv;
+  a.inv_D_lo = (float)(inv - (double)a.inv_D);
+}
+
 template <Src SRC, bool DROP, Out OUT>
 static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_t st) {
   ProfScope ps(SRC == Src::Mix ? "k_stream_norm_fwd" : "k_rms_norm_fwd", st);
@@ -1060,7 +1079,6 @@ static int launch_bwd(const char* what, NormBwd& a, float* scratch, int dtype, c
   RowMap m{256, 1, 0};
   if (np) m = row_map(a.D, vec, np);
   if constexpr (SRC == Src::Mix) {
-    a.tpc = (int)mix_tpc(a.S, m.rpc);
     a.chunks = mix_chunks(a.S, m.rpc);
     a.items *= a.chunks;
   } else {
@@ -1103,7 +1121,7 @@ int stream_norm_fwd_impl(const void* H, const float* H_pre, const void* weight, 
                          float* rstd, int64_t B, int64_t S, int64_t D, int dtype, float eps, cudaStream_t st) {
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = wdtype == MHC_F32; a.sum_out = bi; a.y = y; a.rstd = rstd;
-  a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
+  a.rows = B * S; a.S = S; a.D = D; a.eps = eps; set_inv(a, D);
   return launch_fwd<Src::Mix, false, Out::Plain>("stream_norm_fwd", a, dtype, st);
 }
 
@@ -1124,7 +1142,7 @@ extern "C" int mhc_add_rms_norm_fwd(const void* x, const void* residual, const v
   if (rows == 0 || D == 0) return MHC_OK;
   if (!x || !y) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = y;
-  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
+  a.rstd = rstd; a.rows = rows; a.S = 1; a.D = D; a.eps = eps; set_inv(a, D);
   cudaStream_t st = (cudaStream_t)stream;
   return drop ? launch_fwd<Src::Add, true, Out::Plain>(what, a, dtype, st)
               : launch_fwd<Src::Add, false, Out::Plain>(what, a, dtype, st);
@@ -1141,8 +1159,8 @@ extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, c
   if (!x || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = q;
-  a.scales = scales; a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0;
-  a.rows = rows; a.S = 1; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
+  a.scales = scales; set_group(a, group, D); a.e8m0 = scale_type == MHC_SCALE_E8M0;
+  a.rows = rows; a.S = 1; a.D = D; a.eps = eps; set_inv(a, D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Add, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Add, false, Out::RowScale>(what, a, dtype, st);
@@ -1205,7 +1223,7 @@ extern "C" int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, cons
   if (!H || !H_pre || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
   a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q; a.scales = scales;
-  a.group = (int)group; a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; a.inv_D64 = 1.0 / (double)D; a.inv_D = (float)a.inv_D64;
+  set_group(a, group, D); a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; set_inv(a, D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Mix, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Mix, false, Out::RowScale>(what, a, dtype, st);
