@@ -37,6 +37,7 @@ struct NormFwd {
   int64_t rows, S, D;
   int group, shift;      // columns per scale (GroupScale): 1 << shift
   int G;                 // scales per row
+  int scales8;           // e8m0 scales of 32 columns, 8 at a time on 8 bytes
   int e8m0;
   float eps;
   float inv_D;
@@ -421,9 +422,9 @@ template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, const fl
   }
 }
 
-// From a row's values v (fp32), its sum of squares and, for a scale per row, its largest |v w| to the output: finishes the
-// sums over the row's threads (a barrier), then normalises, scales and stores.  `at` is the element offset of the thread's
-// first pack, DV the row's packs (0: the row does not exist).
+// From a row's values v (fp32; v w for an 8-bit output), its sum of squares and, for a scale per row, its largest |v w| to the
+// output: finishes the sums over the row's threads (a barrier), then normalises, scales and stores.  `at` is the element
+// offset of the thread's first pack, DV the row's packs (0: the row does not exist).
 template <typename T, int V, int NP, Out OUT>
 __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, const Packs<V, NP>& pk, float* sm, int sub, int t,
                                           int DV, int64_t row, int64_t at, float (&v)[NP][V], const float (&w)[NP][V],
@@ -447,13 +448,12 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
       sc = make_scale(mx, rstd, a.e8m0);
       if (DV && t == 0) store_scale(a.scales, row, sc, a.e8m0);
     }
+    if constexpr (OUT == Out::GroupScale) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      g[k] = 0.f;
+      for (int k = 0; k < NP; ++k) {
+        g[k] = 0.f;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[k][e] *= w[k][e];
-        if (OUT == Out::GroupScale) g[k] = max_nan(g[k], fabsf(v[k][e]));
+        for (int e = 0; e < V; ++e) g[k] = max_nan(g[k], fabsf(v[k][e]));
       }
     }
     if constexpr (OUT == Out::GroupScale && V == 1) {   // 64 or 128 columns are 2 or 4 consecutive k of the warp
@@ -473,7 +473,16 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
         for (int o = 16; o > 0; o >>= 1)
           if (V == 1 || o * V < 32 || o * V < a.group) g[k] = max_nan(g[k], __shfl_xor_sync(0xffffffffu, g[k], o));
         sc = make_scale(g[k], rstd, a.e8m0);
-        if (p < DV && (p * V & (a.group - 1)) == 0) store_scale(a.scales, row * a.G + (p * V >> a.shift), sc, a.e8m0);
+        if (V == 8 && a.scales8) {   // a warp's 8 scales as one store: one by one the bytes cost 10 us of 142
+          const int lane = threadIdx.x & 31;
+          const uint32_t c = (p < DV && (lane & 3) == 0) ? sc.code << (8 * ((lane >> 2) & 3)) : 0u;
+          const uint32_t lo = __reduce_or_sync(0xffffffffu, lane < 16 ? c : 0u);
+          const uint32_t hi = __reduce_or_sync(0xffffffffu, lane < 16 ? 0u : c);
+          if (p < DV && lane == 0)
+            *reinterpret_cast<uint2*>((uint8_t*)a.scales + row * a.G + (p >> 2)) = make_uint2(lo, hi);
+        } else if (p < DV && (p * V & (a.group - 1)) == 0) {
+          store_scale(a.scales, row * a.G + (p * V >> a.shift), sc, a.e8m0);
+        }
       }
 #pragma unroll
       for (int e = 0; e < V; ++e) v[k][e] *= sc.f1;
@@ -482,13 +491,14 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
   }
 }
 
-// Adds up a pack's squares and, for a scale per row, its largest |v w|.
+// Adds up a pack's squares; for an 8-bit output v becomes v w, whose largest magnitude a scale per row needs.
 template <int V, Out OUT>
-__device__ __forceinline__ void norm_gather(const float (&v)[V], const float (&w)[V], float& ss, float& mx) {
+__device__ __forceinline__ void norm_gather(float (&v)[V], const float (&w)[V], float& ss, float& mx) {
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     ss = fmaf(v[e], v[e], ss);
-    if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v[e] * w[e]));
+    if (OUT != Out::Plain) v[e] *= w[e];
+    if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v[e]));
   }
 }
 
@@ -1033,10 +1043,13 @@ static int check_quant(const char* what, int64_t group, int scale_type) {
   return MHC_OK;
 }
 
-static void set_group(NormFwd& a, int64_t group, int64_t D) {
+static void set_scales(NormFwd& a, void* scales, int64_t group, int scale_type, int64_t D) {
+  a.scales = scales;
   a.group = (int)group;
   a.shift = group == 32 ? 5 : group == 64 ? 6 : 7;
   a.G = group ? (int)((D + group - 1) / group) : 1;
+  a.e8m0 = scale_type == MHC_SCALE_E8M0;
+  a.scales8 = a.e8m0 && group == 32 && a.G % 8 == 0 && is_aligned_to(a.scales, 8);
 }
 
 static void set_inv(NormFwd& a, int64_t D) {
@@ -1159,7 +1172,7 @@ extern "C" int mhc_add_rms_norm_quant_fwd(const void* x, const void* residual, c
   if (!x || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
   a.x = x; a.res = residual; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.sum_out = sum_out; a.y = q;
-  a.scales = scales; set_group(a, group, D); a.e8m0 = scale_type == MHC_SCALE_E8M0;
+  set_scales(a, scales, group, scale_type, D);
   a.rows = rows; a.S = 1; a.D = D; a.eps = eps; set_inv(a, D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Add, false, Out::GroupScale>(what, a, dtype, st)
@@ -1222,8 +1235,8 @@ extern "C" int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, cons
   if (B == 0 || S == 0 || D == 0) return MHC_OK;
   if (!H || !H_pre || !q || !scales) return fail(MHC_ERR_NULL_POINTER, "%s: null pointer", what);
   NormFwd a{};
-  a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q; a.scales = scales;
-  set_group(a, group, D); a.e8m0 = scale_type == MHC_SCALE_E8M0; a.rows = B * S; a.S = S; a.D = D; a.eps = eps; set_inv(a, D);
+  a.x = H; a.hpre = H_pre; a.weight = weight; a.w_f32 = weight_dtype == MHC_F32; a.y = q;
+  set_scales(a, scales, group, scale_type, D); a.rows = B * S; a.S = S; a.D = D; a.eps = eps; set_inv(a, D);
   cudaStream_t st = (cudaStream_t)stream;
   return group ? launch_fwd<Src::Mix, false, Out::GroupScale>(what, a, dtype, st)
                : launch_fwd<Src::Mix, false, Out::RowScale>(what, a, dtype, st);
