@@ -716,31 +716,36 @@ k_norm_bwd(NormBwd a, RowMap m) {
     if (pk.first + k * pk.step < m.DV) load_w_pack<T, V>(a.weight, a.w_f32, pk.first * V + k * stride, w[k]);
   }
 
-  // where the CTA is: rows base .. base + rpc - 1 of the item, the item's end
-  struct Pos { int64_t item, base, end; };
+  // where the CTA is: rows base .. base + rpc - 1 of the item, the item's end (32 bits: at most 2^31 - 1 rows, and the
+  // counts are unsigned, so that stepping past the last one does not wrap)
+  const uint32_t items = (uint32_t)a.items, chunks = (uint32_t)a.chunks, S = (uint32_t)a.S;
+  struct Pos { uint32_t item, base, end; };
   auto enter = [&](Pos& q) {   // first rows of q.item
-    if (q.item >= a.items) return;
+    if (q.item >= items) return;
     if constexpr (SRC == Src::Mix) {
-      const int64_t b = q.item / a.chunks, c = q.item - b * a.chunks;
-      q.base = b * a.S + c * m.rpc;
-      q.end = (b + 1) * a.S;
+      const uint32_t b = q.item / chunks, c = q.item - b * chunks;
+      q.base = b * S + c * m.rpc;
+      q.end = (b + 1) * S;
     } else {
       q.base = q.item * m.rpc;
-      q.end = min(q.base + m.rpc, a.S);
+      q.end = min(q.base + m.rpc, S);
     }
   };
   auto next = [&](Pos q) -> Pos {
-    q.base += SRC == Src::Mix ? a.chunks * m.rpc : m.rpc;
+    q.base += SRC == Src::Mix ? chunks * m.rpc : m.rpc;
     if (SRC == Src::Add || q.base >= q.end) {
       q.item += gridDim.x;
       enter(q);
     }
     return q;
   };
+  bool own[NP];   // the packs that exist
+#pragma unroll
+  for (int k = 0; k < NP; ++k) own[k] = pk.first + k * pk.step < m.DV;
   auto issue = [&](int stage, const Pos& q) -> float {   // starts the copies of a row; its rstd
-    const int64_t row = q.base + sub;
+    const int64_t row = (int64_t)q.base + sub;
     float rstd = 0.f;
-    if (q.item < a.items && row < q.end) {
+    if (q.item < items && row < q.end) {
       rstd = __ldg(a.rstd + row);
       if constexpr (DEPTH == 0) return rstd;
       const T* src[NS];
@@ -755,7 +760,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
       }
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        if (pk.first + k * pk.step < m.DV) {
+        if (own[k]) {
 #pragma unroll
           for (int n = 0; n < NS; ++n)
             if (SRC == Src::Mix || n < 2 || (n == 2 ? a.res : a.dsum))
@@ -784,10 +789,10 @@ k_norm_bwd(NormBwd a, RowMap m) {
   };
 
   float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  int64_t pre_of = -1;
+  uint32_t pre_of = 0xffffffffu;
   int parity = 0, stage = 0;
   float ahead[DEPTH > 1 ? DEPTH - 1 : 1];   // rstd of the rows on the way
-  Pos q{(int64_t)blockIdx.x, 0, 0};
+  Pos q{blockIdx.x, 0, 0};
   enter(q);
   Pos qi = q;
 #pragma unroll
@@ -795,7 +800,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
     ahead[d] = issue(d, qi);
     qi = next(qi);
   }
-  while (q.item < a.items) {
+  while (q.item < items) {
     float rstd;
     if constexpr (DEPTH <= 1) {
       rstd = issue(0, q);
@@ -808,14 +813,14 @@ k_norm_bwd(NormBwd a, RowMap m) {
       qi = next(qi);
       asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH > 0 ? DEPTH - 1 : 0) : "memory");
     }
-    const int64_t row = q.base + sub;
-    const int DV = row < q.end ? m.DV : 0;
+    const int64_t row = (int64_t)q.base + sub;
+    const bool live = row < q.end;
     const Pos q2 = next(q);
     RawPack<T, V> now[DEPTH == 0 ? NP : 1][3];   // dy, x, residual: all loads before the warp meets over the bits
     if constexpr (DEPTH == 0 && SRC == Src::Add) {
 #pragma unroll
       for (int k = 0; k < NP; ++k)
-        if (pk.first + k * pk.step < DV) {
+        if (live && own[k]) {
           now[k][0] = slot(0, k, 0, row);
           now[k][1] = slot(0, k, 1, row);
           if (a.res) now[k][2] = slot(0, k, 2, row);
@@ -827,7 +832,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
       if (q.item != pre_of) {
         pre_of = q.item;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + q.item / a.chunks * 4 + n);
+        for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + (int64_t)(q.item / chunks) * 4 + n);
       }
     }
     float s[NP][V], h[NP][V], c = 0.f, unused = 0.f;
@@ -835,7 +840,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
     for (int k = 0; k < NP; ++k) {
 #pragma unroll
       for (int e = 0; e < V; ++e) s[k][e] = h[k][e] = 0.f;
-      if (pk.first + k * pk.step < DV) {
+      if (live && own[k]) {
         const RawPack<T, V> dy = DEPTH == 0 && SRC == Src::Add ? now[DEPTH == 0 ? k : 0][0] : slot(stage, k, 0, row);
         if constexpr (SRC == Src::Mix) {
           RawPack<T, V> x[4];
@@ -855,22 +860,22 @@ k_norm_bwd(NormBwd a, RowMap m) {
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float g = raw_get<V>(dy, e);
+          const float g = raw_get<V>(dy, e) * rstd;
           h[k][e] = g * w[k][e];
           c = fmaf(h[k][e], s[k][e], c);
-          dw[k][e] = fmaf(g, s[k][e] * rstd, dw[k][e]);
+          dw[k][e] = fmaf(g, s[k][e], dw[k][e]);
         }
       }
     }
     row_sum_max<false>(c, unused, sm[parity], m, sub);
     parity ^= 1;   // the next row's sums go to the other half: nobody can still be reading it
-    const float kk = c * rstd * rstd * rstd * a.inv_D;
+    const float kk = c * rstd * rstd * a.inv_D;   // c holds one rstd already
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-      if (pk.first + k * pk.step < DV) {
+      if (live && own[k]) {
         float g[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[e] = rstd * h[k][e] - s[k][e] * kk;
+        for (int e = 0; e < V; ++e) g[e] = fmaf(-kk, s[k][e], h[k][e]);
         if constexpr (SRC == Src::Mix) {
           T* o = (T*)a.dx + row * 4 * D + pk.first * V + k * stride;
 #pragma unroll
@@ -901,7 +906,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
     if constexpr (SRC == Src::Mix) {
       if (q2.item != q.item) {
         __syncthreads();   // the previous item's readers of red are done
-        block_reduce_store<4>(acc, a.dpre_part + q.item * 4, red);
+        block_reduce_store<4>(acc, a.dpre_part + (int64_t)q.item * 4, red);
 #pragma unroll
         for (int n = 0; n < 4; ++n) acc[n] = 0.f;
       }
