@@ -202,7 +202,7 @@ def add_residual_dropout_backward(dH_new, branch_output, H_post, rng, threshold:
     buf, nbytes = L.scratch(L.OP_ADD_RESIDUAL_BWD, B, S, D, dH_new)
     L.call_on(dev, "mhc_add_residual_dropout_bwd", dH_new.data_ptr(), branch_output.data_ptr(), H_post.data_ptr(),
               rng.data_ptr(), threshold, row_offset, d_bo.data_ptr(), dH_post.data_ptr(), buf.data_ptr(), nbytes,
-              L.tickets(dH_new, B), B, S, D, L.dtype_code(dH_new))
+              L.eager_tickets(dH_new, B), B, S, D, L.dtype_code(dH_new))
     return dH_new, d_bo, dH_post
 
 

@@ -317,7 +317,7 @@ def _scales_for(lead, D, group, scale_dtype, device):
         raise ValueError(f"group must be None (one scale per row), 32, 64 or 128, got {group}")
     if scale_dtype not in _SCALES:
         raise TypeError(f"mhc: unsupported scale dtype {scale_dtype} (float32, float8_e8m0fnu only)")
-    G = -(-D // group) if group else 1
+    G = -(-D // group) if group else min(D, 1)
     return group, _SCALES[scale_dtype], torch.empty((*lead, G), device=device, dtype=scale_dtype)
 
 
@@ -400,5 +400,5 @@ def hc_mix_norm_forward(H, H_pre_base, H_post_base, H_res_base, phi, alpha_pre, 
     L.call_on(index, "mhc_hc_mix_norm_fwd", L.ptr(H), L.ptr(phi), L.ptr(pre_b), L.ptr(post_b), L.ptr(res_b), L.ptr(a[0]),
               L.ptr(a[1]), L.ptr(a[2]), wptr, wcode, float(norm_eps), L.ptr(x), L.ptr(H_pre), L.ptr(H_post),
               L.ptr(H_res), L.ptr(saved), L.ptr(bi), L.ptr(y), L.ptr(rstd), L.ptr(pooled), chunks, L.ptr(buf), nbytes,
-              L.tickets(H, B), B, S, D, L.dtype_code(H), int(sinkhorn_iters), float(eps))
+              L.eager_tickets(H, B), B, S, D, L.dtype_code(H), int(sinkhorn_iters), float(eps))
     return y, bi, rstd, H_post, H_pre, H_res, x, saved

@@ -230,6 +230,12 @@ def tickets(like: torch.Tensor, n: int):
     return buf.data_ptr()
 
 
+def eager_tickets(like: torch.Tensor, n: int):
+    """`tickets`, but none while a CUDA graph is captured: graphs captured on one stream would share its counters and
+    could be replayed at the same time."""
+    return None if torch.cuda.is_current_stream_capturing() else tickets(like, n)
+
+
 def f32c(t: torch.Tensor) -> torch.Tensor:
     """fp32, contiguous view or copy."""
     if t.dtype != torch.float32:

@@ -333,7 +333,7 @@ def _add_rms_norm_quant_fwd(x: Tensor, residual: Optional[Tensor], weight: Optio
 @_add_rms_norm_quant_fwd.register_fake
 def _(x, residual, weight, eps, group, scale_dtype):
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
-    G = -(-x.shape[-1] // group) if group else 1
+    G = -(-x.shape[-1] // group) if group else torch.sym_min(x.shape[-1], 1)
     return (q, x.new_empty(tuple(x.shape[:-1]) + (G,), dtype=scale_dtype),
             torch.empty_like(x, memory_format=torch.contiguous_format) if residual is not None else x.new_empty(0))
 
@@ -386,7 +386,7 @@ def _stream_norm_quant_fwd(H: Tensor, H_pre: Tensor, weight: Optional[Tensor], e
 @_stream_norm_quant_fwd.register_fake
 def _(H, H_pre, weight, eps, group, scale_dtype):
     Bn, S, _, D = H.shape
-    G = -(-D // group) if group else 1
+    G = -(-D // group) if group else torch.sym_min(D, 1)
     return H.new_empty(Bn, S, D, dtype=torch.float8_e4m3fn), H.new_empty(Bn, S, G, dtype=scale_dtype)
 
 

@@ -471,9 +471,9 @@ def test_two_layer_stack_against_64_bits():
         keep = SO.keep_mask(8, i, B * S, D, p).view(B, S, D)
         z = torch.einsum("bnm,bsmd->bsnd", R, z) + post[:, None, :, None] * SO.dropout(torch.sin(y), keep, p).unsqueeze(2)
     z.backward(g.double())
-    for a, b in ((x, z), (H.grad, H64.grad), (wl[0].grad, w64[0].grad), (wl[1].grad, w64[1].grad)):
+    for a, b in ((x.detach(), z.detach()), (H.grad, H64.grad), (wl[0].grad, w64[0].grad), (wl[1].grad, w64[1].grad)):
         # fp32 chains of a few hundred roundings, largest entries a few times the typical one: 1e-5 of the largest
-        assert float((a.detach().double().cpu() - b.detach()).abs().max()) <= 1e-5 * float(b.abs().max())
+        assert float((a.double().cpu() - b).abs().max()) <= 1e-5 * float(b.abs().max())
 
 
 def test_gradient_of_the_kernels_against_differences():
@@ -534,6 +534,49 @@ def test_empty_inputs():
     out = mhc.fused_stream_norm(H, pre, w)
     gH, gp, gw = torch.autograd.grad(out, [H, pre, w], torch.empty_like(out))
     assert gH.shape == H.shape and torch.equal(gp, torch.zeros_like(pre)) and torch.equal(gw, torch.zeros_like(w))
+
+
+def test_no_columns():
+    import mhc
+    x = torch.empty(3, 0, device="cuda", requires_grad=True)
+    y, _ = mhc.fused_add_rms_norm(x, torch.empty(3, 0, device="cuda"), torch.empty(0, device="cuda"))
+    assert torch.autograd.grad(y.sum(), x)[0].shape == (3, 0)
+    q, s, _ = mhc.fused_add_rms_norm_quant(x.detach())
+    assert q.shape == (3, 0) and s.shape == (3, 0)
+    assert mhc.counter_dropout(x, 0.5, rng=(1, 1)).shape == (3, 0)
+
+
+def test_one_tensor_as_input_and_residual():
+    import mhc
+    torch.manual_seed(0)
+    x, w, dy, ds = torch.randn(40, 256), torch.rand(256) + 0.5, torch.randn(40, 256), torch.randn(40, 256)
+    leaf = x.cuda().requires_grad_(True)
+    y, s = mhc.fused_add_rms_norm(leaf, leaf, w.cuda(), EPS)
+    (g,) = torch.autograd.grad([y, s], [leaf], [dy.cuda(), ds.cuda()])
+    s64 = 2 * x.double()
+    _, rstd = SO.rms_norm(s64, w.double(), EPS)
+    g64, _, g_mag, _ = SO.rms_norm_grad(dy.double(), s64, rstd, w.double())
+    within(g, 2 * (g64 + ds.double()), 4 * steps(256) * U * (g_mag + ds.double().abs()), "dx")
+
+
+def test_norm_weight_beside_a_gradient_record():
+    """A layer whose parameter gradients go to a GradSync record still returns the norm weight's gradient."""
+    import mhc
+    B, S, D = 2, 16, 128
+    H0, g = torch.randn(B, S, 4, D, device="cuda"), torch.randn(B, S, 4, D, device="cuda")
+    w0 = torch.rand(D, device="cuda") + 0.5
+    got = []
+    for sync in (False, True):
+        hc = layer(D)
+        gs = mhc.GradSync([hc]) if sync else None
+        H, w = H0.clone().requires_grad_(True), w0.clone().requires_grad_(True)
+        y, add = hc(H, w)
+        add(torch.sin(y), dropout_p=0.2, rng=(1, 2)).backward(g)
+        if sync:
+            gs.finish()
+        got.append([H.grad, w.grad, *[p.grad.clone() for p in hc.parameters()]])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
 
 
 def test_only_some_gradients_are_wanted():
@@ -609,6 +652,67 @@ def test_captured_step_follows_the_generator_state():
             assert torch.equal(a, b)
         seen.append(got[0])
     assert not torch.equal(seen[0], seen[1])
+
+
+def test_captured_draw_from_torchs_generator():
+    """rng=None in a graph: every replay draws anew, and the backward of a replay uses that replay's mask."""
+    import mhc
+    x = torch.rand(64, 256, device="cuda") + 1
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        y = mhc.counter_dropout(leaf, 0.4)
+        return y.detach(), torch.autograd.grad(y, leaf, torch.ones_like(x))[0]
+
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, g = step()
+    masks = []
+    for _ in range(2):
+        graph.replay()
+        assert torch.equal(y != 0, g != 0)
+        masks.append((y != 0).clone())
+    assert not torch.equal(*masks)
+
+
+def test_two_graphs_of_one_stream_replayed_together():
+    """Backwards with dropout captured one after the other share nothing that replaying them at once would upset."""
+    import mhc
+    B, S, D = 2, 256, 1024
+    data = [[torch.randn(B, S, 4, D, device="cuda"), torch.randn(B, S, D, device="cuda"), torch.rand(B, 4, device="cuda")]
+            for _ in range(2)]
+    rng = torch.tensor([1, 2], device="cuda")
+    stream = torch.cuda.Stream()
+
+    def step(d):
+        leaves = [t.detach().requires_grad_(True) for t in d]
+        out = mhc.fused_add_residual(*leaves, dropout_p=0.3, rng=rng)
+        return torch.autograd.grad(out, leaves[1:], d[0])
+
+    with torch.cuda.stream(stream):
+        want = [[t.clone() for t in step(d)] for d in data]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for d in data:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs.append(step(d))
+        graphs.append(graph)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for graph, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for out, ref in zip(outs, want):
+        for a, b in zip(out, ref):
+            assert torch.equal(a, b)
 
 
 def test_checkpointing_recomputes_the_same_mask():
