@@ -164,7 +164,7 @@ __device__ __forceinline__ void block_sum_max(float& sum, float& mx, float* sm) 
   mx = m;
 }
 
-// ------------------------------------------------------------------------------------- any width, any alignment
+// -------------------------------------------------------- rows too wide for registers (over 16384, or 8192 odd or unaligned)
 // s[row, d], read element by element.
 template <typename T, Src SRC, bool DROP>
 __device__ __forceinline__ float src_at(const NormFwd& a, const DropSeed& seed, const float (&pre)[4], int64_t row, int64_t d) {
@@ -243,7 +243,7 @@ k_norm_any_fwd(NormFwd a) {
   }
 }
 
-// Persistent CTAs of 256 threads: CTA i takes items i, i + grid, ...  An item is a row (Add), or a chunk of tokens of
+// Persistent CTAs of 256 threads: CTA i takes items i, i + grid, ...  An item is a row (Add), or a share of the tokens of
 // one batch element (Mix), whose dH_pre it sums.  dweight's partial sums live in the CTA's own row of dw_part.
 template <typename T, Src SRC, bool DROP>
 __global__ void __launch_bounds__(256)
@@ -309,7 +309,7 @@ k_norm_any_bwd(NormBwd a) {
   }
 }
 
-// ------------------------------------------------------------------ rows that divide into 16-byte packs, in registers
+// --------------------------------------------------------------------------------------------- rows held in registers
 // A row belongs to `tpr` threads (a multiple of 32) that own NP packs each, all loaded before the first use and kept in
 // registers as fp32 between the row sum and the output, so the data is read once.  Narrow rows share a CTA of 256
 // threads.  Bound by memory; the one barrier of a row is covered by the other CTAs.
@@ -510,7 +510,8 @@ __device__ __forceinline__ void mix_pack(const RawPack<T, V> (&x)[4], const floa
            pre[3] * raw_get<V>(x[3], e);
 }
 
-// One row per thread group, once.
+// One row per thread group, once: bound by memory (162 us at 32768 x 4096 bf16 with a residual and the sum written, four
+// tensors = 6.6 TB/s), for the many CTAs an SM holds and their short lives; a persistent form of it took 176.
 template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
 __global__ void __launch_bounds__(V == 1 ? 1024 : 512, NP == 2 ? 2 : 1)
 k_norm_fwd(NormFwd a, RowMap m) {
@@ -584,8 +585,10 @@ k_norm_fwd(NormFwd a, RowMap m) {
   norm_emit<T, V, NP, OUT>(a, m, pk, sm, sub, t, DV, row, at, v, w, ss, mx);
 }
 
-// Many rows and more to do per pack than to add, norm and store it (8-bit output, dropout): persistent CTAs that keep the weight and the columns' part of the generator in registers, with the next row's
-// packs on the way by cp.async into slots of shared memory that only the thread itself reads.
+// Many rows and more to do per pack than to add, norm and store it (8-bit output, dropout): persistent CTAs that keep the
+// weight and the columns' part of the generator in registers, with the next row's packs on the way by cp.async into slots of
+// shared memory that only the thread itself reads.  The one-shot form is bound by instructions there: 16384 x 7168 bf16 to
+// e4m3 with a scale per 32 columns 170 us against 132 (6.2 TB/s), 8192 x 7168 with dropout 90 against 82.
 template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
 __global__ void __launch_bounds__(512, 2)
 k_norm_fwd_ring(NormFwd a, RowMap m) {
@@ -690,7 +693,10 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
 // dweight's running sums in registers.  The packs of the next DEPTH - 1 rows are on the way meanwhile, by cp.async into
 // slots of shared memory that only the thread itself reads (no barrier): in registers they spilled, and the
 // stream form ran at 42 % of the memory's rate.  An item is rpc rows (Add) or one of `chunks` shares of a batch element's
-// tokens (Mix): every chunks-th group of rpc tokens, so that the CTAs sweep the memory side by side.  DEPTH 0 (single elements, which cp.async cannot copy): loads straight from memory.
+// tokens (Mix): every chunks-th group of rpc tokens, so that the CTAs sweep the memory side by side.  DEPTH 0 (single
+// elements, which cp.async cannot copy): loads straight from memory.  204 us at 32768 x 4096 bf16 (five tensors, 6.6 TB/s),
+// 118 at 8192 x 7168 with dropout (six, 6.0 TB/s, bound by instructions: 14 warps per SM and twice as many per pack), 108
+// for the streams at 2 x 4096 x 4096 (nine, 5.6 TB/s).  One pack per thread and twice the warps was no faster.
 template <typename T, int V, int NP, int DEPTH, int THREADS, Src SRC, bool DROP>
 __global__ void __launch_bounds__(THREADS)
 k_norm_bwd(NormBwd a, RowMap m) {
@@ -930,7 +936,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
   }
 }
 
-// Ends the backward, both sums in fp64 and a fixed order.  CTAs [0, wide): out[d] = sum_i part[i, d], 32 columns per CTA, 32
+// Ends the backward in 3 us (296 partial rows of 4096), both sums in fp64 and a fixed order.  CTAs [0, wide): out[d] = sum_i part[i, d], 32 columns per CTA, 32
 // threads per column that take rows i, i + 32, ...  CTA wide + b: dH_pre[b] from its chunks' four sums.
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -987,9 +993,10 @@ static int64_t mix_chunks(int64_t S, int rpc) {
   return groups <= 4 ? (groups > 0 ? 1 : 0) : few < most ? few : most;
 }
 
-#ifndef MHC_RING_MIN
-#define MHC_RING_MIN 4
-#endif
+// Rows per CTA from which the persistent forward is taken: at 4 the two forms take the same time (1184 x 7168: 15 us,
+// 2368 x 4096: 16 us, either way), below it the one-shot form is up to half a microsecond faster, and at 4736 x 7168
+// the persistent one takes 44 us against 55.
+constexpr int kRingRows = 4;
 // Shared memory of an SM that the resident CTAs' rings may use together (each has a few hundred bytes of its own beside).
 constexpr size_t kRingBytes = 224 * 1024;
 
@@ -1076,7 +1083,7 @@ static int launch_fwd(const char* what, const NormFwd& a, int dtype, cudaStream_
   const unsigned grid = (unsigned)((a.rows + m.rpc - 1) / m.rpc), block = (unsigned)(m.tpr * m.rpc);
   const size_t smem = (size_t)2 * block * np * (SRC == Src::Mix ? 4 : 2) * 16;
   const int per_sm = std::min(1024 / (int)block, (int)(kRingBytes / smem));
-  if ((DROP || OUT != Out::Plain) && np == 2 && per_sm > 0 && grid >= (unsigned)(MHC_RING_MIN * per_sm * sm_count())) {
+  if ((DROP || OUT != Out::Plain) && np == 2 && per_sm > 0 && grid >= (unsigned)(kRingRows * per_sm * sm_count())) {
     MHC_TYPE_DISPATCH(dtype, (launch_ring<k_norm_fwd_ring<T, vec_width<T>::value, 2, SRC, DROP, OUT>>((unsigned)(per_sm * sm_count()),
                                           block, smem, st, a, m)));
     return check_launch(what);
