@@ -127,6 +127,9 @@ __device__ __forceinline__ Scale make_scale(float umax, const Rstd2& rstd, int e
     if (s < kMinScale) {  // false for NaN
       r.f32 = kMinScale;
       r.f2 = 8.50705917302346159e37f;   // 2^126
+    } else if (umax < 1.2e-35f) {   // 448 / umax could overflow where rstd is large; amax is not below 448 * 2^-126
+      r.f32 = s;
+      r.f2 = __fdiv_rn(kE4m3Max, amax);
     } else {
       r.f32 = s;
       r.f1 = __fdiv_rn(kE4m3Max, umax);
@@ -936,8 +939,9 @@ k_norm_bwd(NormBwd a, RowMap m) {
   }
 }
 
-// Ends the backward in 3 us (296 partial rows of 4096), both sums in fp64 and a fixed order.  CTAs [0, wide): out[d] = sum_i part[i, d], 32 columns per CTA, 32
-// threads per column that take rows i, i + 32, ...  CTA wide + b: dH_pre[b] from its chunks' four sums.
+// Ends the backward in 3 us (296 partial rows of 4096), both sums in fp64 and a fixed order.  CTAs [0, wide): out[d] =
+// sum_i part[i, d], 32 columns per CTA, 32 threads per column that take rows i, i + 32, ...  CTA wide + b: dH_pre[b] from
+// its chunks' four sums.
 template <typename T>
 __global__ void __launch_bounds__(1024)
 k_norm_finish(const float* __restrict__ part, int n, int64_t D, T* __restrict__ out, int wide,

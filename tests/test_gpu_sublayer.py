@@ -264,6 +264,24 @@ def test_stream_norm_quant(B, S, D, dt, group, e8m0):
     check_quant(q, scales, y64, steps(D) * U * (1 + row) * rstd * w.double().abs() * b_mag + 1e-300, group, e8m0, D)
 
 
+# Enough rows for the persistent forward (4 per resident block): narrow rows that share a block, rows of a few warps, wide ones;
+# counts that do not divide.
+@pytest.mark.parametrize("rows,D", [(19013, 40), (9601, 584), (2407, 4096), (1201, 7168)])
+def test_many_rows(rows, D):
+    test_add_rms_norm(rows, D, "bf16", "f32", True, 0.1)
+    test_add_rms_norm(rows, D, "f16", "f16", False, 0.5)
+    test_add_rms_norm_quant(rows, D, "bf16", "bf16", True, 32, True)
+    test_add_rms_norm_quant(rows, D, "f16", "f32", False, 128, False)
+    test_add_rms_norm_quant(rows, D, "bf16", None, True, 0, False)
+
+
+@pytest.mark.parametrize("B,S,D", [(3, 3201, 584), (5, 482, 4096)])
+def test_many_tokens(B, S, D):
+    test_stream_norm_quant(B, S, D, "bf16", 32, True)
+    test_stream_norm_quant(B, S, D, "f16", 0, False)
+    test_stream_norm(B, S, D, "bf16", "f32")
+
+
 def test_norm_of_infinities_and_nan_stays_in_its_row():
     import mhc
     x = draw((6, 512), torch.bfloat16, 1)
@@ -299,6 +317,20 @@ def test_zero_rows_and_tiny_values_in_8_bits():
             assert (s[0] == SO.MIN_SCALE).all() and (q.float().cpu()[0] == 0).all()
             back = q.double().cpu()[1] * s[1].repeat_interleave(group or 256)
             assert ((back - 1e-27).abs() <= 1e-27 / 16 * 1.01).all()
+
+
+@pytest.mark.parametrize("size", [1e-20, 1e-34, 3e-36, 2e-37, 3e-38])
+@pytest.mark.parametrize("group", [0, 32])
+@pytest.mark.parametrize("e8m0", [False, True])
+def test_rows_near_the_smallest_numbers_in_8_bits(size, group, e8m0):
+    """rstd is 1000 there (eps): the values are normal numbers, their inputs' reciprocals are not."""
+    import mhc
+    x = draw((5, 256), torch.float32, 7) * size
+    x = torch.where(x.abs() < 1.2e-38, torch.zeros(()), x)       # no subnormal inputs
+    q, scales, _ = mhc.fused_add_rms_norm_quant(*cuda(x, None, torch.ones(256)), EPS, group=group or None,
+                                                scale_dtype=torch.float8_e8m0fnu if e8m0 else torch.float32)
+    y64, _ = SO.rms_norm(x.double(), torch.ones(256, dtype=torch.float64), EPS)
+    check_quant(q, scales, y64, 2 * steps(256) * U * y64.abs() + 1e-300, group, e8m0, 256)
 
 
 # ------------------------------------------------------------------------------------------------ dropout
@@ -771,6 +803,28 @@ def test_many_rows_past_32_bit_offsets():
     d = mhc.counter_dropout(x, 0.5, rng=(1, 2))
     keep = SO.keep_mask(1, 2, 3, D, 0.5, rows - 3)
     assert torch.equal(d[-3:].cpu(), torch.where(keep, x[-3:].float().cpu() * 2, torch.zeros(())).bfloat16())
+    q, scales, _ = mhc.fused_add_rms_norm_quant(x, None, w, group=32, scale_dtype=torch.float8_e8m0fnu)
+    check_quant(q[-3:], scales[-3:], y64, 2 * steps(D) * U * y64.abs() + 1e-300, 32, True, D)
+    del q, scales, y
+    leaf = x.requires_grad_(True)
+    out, _ = mhc.fused_add_rms_norm(leaf, None, w)
+    (dx,) = torch.autograd.grad(out, leaf, d)
+    dy = d[-3:].double().cpu()
+    _, rstd = SO.rms_norm(tail, torch.ones(D, dtype=torch.float64), EPS)
+    g64, _, g_mag, _ = SO.rms_norm_grad(dy, tail, rstd, torch.ones(D, dtype=torch.float64))
+    within(dx[-3:], g64, 2.0 ** -8 * g64.abs() + 2 * steps(D) * U * g_mag + 1e-30, "dx tail")
+    del dx, out, d
+    H, pre = x.detach()[:269996].view(1, 67499, 4, D).requires_grad_(True), torch.tensor([[0.1, 0.2, 0.3, 0.4]], device="cuda")
+    b64, b_mag = mixed64(H[:, -2:].detach().cpu(), pre.cpu())
+    y64, rstd = SO.rms_norm(b64, torch.ones(D, dtype=torch.float64), EPS)
+    y = mhc.fused_stream_norm(H, pre, w)
+    within(y[:, -2:], y64, 2.0 ** -8 * y64.abs() + 4 * steps(D) * U * rstd * b_mag + 1e-30, "stream tail")
+    (dH,) = torch.autograd.grad(y, H, y.detach())
+    dy = y[:, -2:].detach().double().cpu()
+    g64, _, g_mag, _ = SO.rms_norm_grad(dy, b64, rstd, torch.ones(D, dtype=torch.float64))
+    p64 = pre.double().cpu()[:, None, :, None]
+    within(dH[:, -2:], p64 * g64.unsqueeze(2), p64 * (2.0 ** -8 * g64.abs() + 8 * steps(D) * U * (g_mag + rstd ** 2 * b_mag)
+                                                      ).unsqueeze(2) + 1e-30, "dH tail")
 
 
 def test_kernels_are_the_librarys_own():
