@@ -781,20 +781,14 @@ k_norm_bwd(NormBwd a, RowMap m) {
     if constexpr (DEPTH > 0) asm volatile("cp.async.commit_group;" ::: "memory");
     return rstd;
   };
-  auto slot = [&](int stage, int k, int n, int64_t row) -> RawPack<T, V> {
-    if constexpr (DEPTH == 0) {
-      const T* src = n == 0 ? (const T*)a.dy + row * D
-                   : SRC == Src::Mix ? (const T*)a.x + (row * 4 + n - 1) * D
-                   : (const T*)(n == 1 ? a.x : n == 2 ? a.res : a.dsum) + row * D;
-      return ld_raw<T, V>(src + pk.first * V + k * stride);
-    } else {
-      RawPack<T, V> r;
+  auto slot = [&](int stage, int k, int n) -> RawPack<T, V> {
+    RawPack<T, V> r;
+    if constexpr (DEPTH > 0)
       asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                    : "=r"(r.w.x), "=r"(r.w.y), "=r"(r.w.z), "=r"(r.w.w)
                    : "r"(mine + (uint32_t)((stage * NP + k) * NS + n) * pitch)
                    : "memory");
-      return r;
-    }
+    return r;
   };
 
   float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -825,16 +819,35 @@ k_norm_bwd(NormBwd a, RowMap m) {
     const int64_t row = (int64_t)q.base + sub;
     const bool live = row < q.end;
     const Pos q2 = next(q);
-    RawPack<T, V> now[DEPTH == 0 ? NP : 1][3];   // dy, x, residual: all loads before the warp meets over the bits
-    if constexpr (DEPTH == 0 && SRC == Src::Add) {
+    RawPack<T, V> now[DEPTH == 0 ? NP : 1][NS];
+    if constexpr (DEPTH == 0) {   // all at once and without a branch: what does not exist reads the first column of a row that does
+      const int64_t r = live ? row : (int64_t)q.base;
 #pragma unroll
-      for (int k = 0; k < NP; ++k)
-        if (live && own[k]) {
-          now[k][0] = slot(0, k, 0, row);
-          now[k][1] = slot(0, k, 1, row);
-          if (a.res) now[k][2] = slot(0, k, 2, row);
+      for (int k = 0; k < NP; ++k) {
+        const int64_t at = own[k] ? pk.first + k * pk.step : 0;
+        now[k][0] = ld_raw<T, V>((const T*)a.dy + r * D + at);
+        if constexpr (SRC == Src::Mix) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) now[k][1 + n] = ld_raw<T, V>((const T*)a.x + (r * 4 + n) * D + at);
+        } else {
+          now[k][1] = ld_raw<T, V>((const T*)a.x + r * D + at);
         }
+      }
+      if constexpr (SRC == Src::Add) {
+        if (a.res) {
+#pragma unroll
+          for (int k = 0; k < NP; ++k) now[k][2] = ld_raw<T, V>((const T*)a.res + r * D + (own[k] ? pk.first + k * pk.step : 0));
+        }
+        if (a.dsum) {
+#pragma unroll
+          for (int k = 0; k < NP; ++k) now[k][3] = ld_raw<T, V>((const T*)a.dsum + r * D + (own[k] ? pk.first + k * pk.step : 0));
+        }
+      }
     }
+    auto pack = [&](int k, int n) -> RawPack<T, V> {
+      if constexpr (DEPTH == 0) return now[k][n];
+      else return slot(stage, k, n);
+    };
     DropBits<V> bits[DROP ? NP : 1];
     if constexpr (DROP) drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, exchange, bits);
     if constexpr (SRC == Src::Mix) {
@@ -849,27 +862,30 @@ k_norm_bwd(NormBwd a, RowMap m) {
     for (int k = 0; k < NP; ++k) {
 #pragma unroll
       for (int e = 0; e < V; ++e) s[k][e] = h[k][e] = 0.f;
-      if (live && own[k]) {
-        const RawPack<T, V> dy = DEPTH == 0 && SRC == Src::Add ? now[DEPTH == 0 ? k : 0][0] : slot(stage, k, 0, row);
+      // single elements: selected below; a branch here held their loads back (457 -> 271 us at 16384 x 4095 fp32)
+      constexpr bool kSelect = DEPTH == 0 && !DROP;
+      if (kSelect || (live && own[k])) {
+        const RawPack<T, V> dy = pack(k, 0);
         if constexpr (SRC == Src::Mix) {
           RawPack<T, V> x[4];
 #pragma unroll
-          for (int n = 0; n < 4; ++n) x[n] = slot(stage, k, 1 + n, row);
+          for (int n = 0; n < 4; ++n) x[n] = pack(k, 1 + n);
           mix_pack<T, V>(x, pre, s[k]);
         } else {
-          const RawPack<T, V> x = DEPTH == 0 ? now[DEPTH == 0 ? k : 0][1] : slot(stage, k, 1, row);
+          const RawPack<T, V> x = pack(k, 1);
 #pragma unroll
           for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(x, e);
           if constexpr (DROP) drop_apply<V>(a.drop, bits[k], s[k]);
           if (a.res) {
-            const RawPack<T, V> r = DEPTH == 0 ? now[DEPTH == 0 ? k : 0][2] : slot(stage, k, 2, row);
+            const RawPack<T, V> r = pack(k, 2);
 #pragma unroll
             for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r, e);
           }
         }
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const float g = raw_get<V>(dy, e) * rstd;
+          float g = raw_get<V>(dy, e) * rstd;
+          if (kSelect && !(live && own[k])) g = s[k][e] = 0.f;
           h[k][e] = g * w[k][e];
           c = fmaf(h[k][e], s[k][e], c);
           dw[k][e] = fmaf(g, s[k][e], dw[k][e]);
@@ -889,7 +905,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
           T* o = (T*)a.dx + row * 4 * D + pk.first * V + k * stride;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const RawPack<T, V> x = slot(stage, k, 1 + n, row);
+            const RawPack<T, V> x = pack(k, 1 + n);
             float u[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
@@ -900,7 +916,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
           }
         } else {
           if (a.dsum) {
-            const RawPack<T, V> ds = slot(stage, k, 3, row);
+            const RawPack<T, V> ds = pack(k, 3);
 #pragma unroll
             for (int e = 0; e < V; ++e) g[e] += raw_get<V>(ds, e);
           }
