@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "mhc", "libmhc_b200.so")
 SOURCES = ["api.cu", "sinkhorn.cu", "stream.cu", "weights.cu", "weights_rows.cu", "weights_rows_tc.cu", "fused.cu", "noalloc.cu",
            "norm.cu", "dropout.cu"]
-HEADERS = ["common.cuh", "launch.h", "rng.cuh", os.path.join("..", "..", "include", "mhc_b200.h")]
+HEADERS = ["common.cuh", "launch.h", "rng.cuh", "pairs.cuh", os.path.join("..", "..", "include", "mhc_b200.h")]
 
 
 def nvcc_path():

@@ -14,6 +14,7 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "pairs.cuh"
 #include "rng.cuh"
 
 namespace mhc {
@@ -64,6 +65,11 @@ struct NormBwd {
   float inv_D;
   Drop drop;
 };
+
+template <typename T, int V> __device__ __forceinline__ void unpack(const RawPack<T, V>& r, float (&o)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = raw_get<V>(r, e);
+}
 
 template <typename T> __device__ __forceinline__ float load_w(const void* w, int w_f32, int64_t d) {
   if (!w) return 1.f;
@@ -412,14 +418,15 @@ __device__ __forceinline__ void load_w_pack(const void* w, int w_f32, int col, f
   }
 }
 
-template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, const float (&u)[V], float f) {
+template <int V> __device__ __forceinline__ void store_e4m3(uint8_t* p, float (&u)[V], float f) {
+  pack_scale<V>(u, f);
   if constexpr (V == 1) {
-    *p = (uint8_t)e4m3x2(u[0] * f, 0.f);
+    *p = (uint8_t)e4m3x2(u[0], 0.f);
   } else {
     uint32_t w[V / 4];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i)
-      w[i] = (uint32_t)e4m3x2(u[4 * i] * f, u[4 * i + 1] * f) | ((uint32_t)e4m3x2(u[4 * i + 2] * f, u[4 * i + 3] * f) << 16);
+      w[i] = (uint32_t)e4m3x2(u[4 * i], u[4 * i + 1]) | ((uint32_t)e4m3x2(u[4 * i + 2], u[4 * i + 3]) << 16);
     if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
     else *reinterpret_cast<uint32_t*>(p) = w[0];
   }
@@ -439,8 +446,8 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
     if (a.rstd && DV && t == 0) a.rstd[row] = rstd;
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[k][e] = v[k][e] * rstd * w[k][e];
+      pack_scale<V>(v[k], rstd);
+      pack_mul<V>(v[k], w[k]);
       if (pk.first + k * pk.step < DV) PackIO<T, V>::store((T*)a.y + at + k * stride, v[k]);
     }
   } else {
@@ -487,8 +494,7 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
           store_scale(a.scales, row * a.G + (p * V >> a.shift), sc, a.e8m0);
         }
       }
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[k][e] *= sc.f1;
+      pack_scale<V>(v[k], sc.f1);
       if (p < DV) store_e4m3<V>((uint8_t*)a.y + at + k * stride, v[k], sc.f2);
     }
   }
@@ -496,21 +502,31 @@ __device__ __forceinline__ void norm_emit(const NormFwd& a, const RowMap& m, con
 
 // Adds up a pack's squares; for an 8-bit output v becomes v w, whose largest magnitude a scale per row needs.
 template <int V, Out OUT>
-__device__ __forceinline__ void norm_gather(float (&v)[V], const float (&w)[V], float& ss, float& mx) {
+__device__ __forceinline__ void norm_gather(float (&v)[V], const float (&w)[V], Sum2& ss, float& mx) {
+  pack_dot<V>(ss, v, v);
+  if (OUT != Out::Plain) pack_mul<V>(v, w);
+  if (OUT == Out::RowScale) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    ss = fmaf(v[e], v[e], ss);
-    if (OUT != Out::Plain) v[e] *= w[e];
-    if (OUT == Out::RowScale) mx = max_nan(mx, fabsf(v[e]));
+    for (int e = 0; e < V; ++e) mx = max_nan(mx, fabsf(v[e]));
   }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void mix_pack(const RawPack<T, V> (&x)[4], const float (&pre)[4], float (&v)[V]) {
+  float u[V];
+  unpack<T, V>(x[0], v);
+  pack_scale<V>(v, pre[0]);
 #pragma unroll
-  for (int e = 0; e < V; ++e)
-    v[e] = ((pre[0] * raw_get<V>(x[0], e) + pre[1] * raw_get<V>(x[1], e)) + pre[2] * raw_get<V>(x[2], e)) +
-           pre[3] * raw_get<V>(x[3], e);
+  for (int n = 1; n < 4; ++n) {
+    const float p[2] = {pre[n], pre[n]};
+    unpack<T, V>(x[n], u);
+    if constexpr (V == 1) {
+      v[0] = fmaf(p[0], u[0], v[0]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e += 2) unpair(fma2(pair(p[0], p[1]), pair(u[e], u[e + 1]), pair(v[e], v[e + 1])), v[e], v[e + 1]);
+    }
+  }
 }
 
 // One row per thread group, once: bound by memory (162 us at 32768 x 4096 bf16 with a residual and the sum written, four
@@ -566,7 +582,8 @@ k_norm_fwd(NormFwd a, RowMap m) {
     drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, exchange, bits);
   }
   T* so = (T*)a.sum_out + at;
-  float v[NP][V], ss = 0.f, mx = 0.f;
+  float v[NP][V], mx = 0.f;
+  Sum2 ss{0};
 #pragma unroll
   for (int k = 0; k < NP; ++k) {
     const bool ok = pk.first + k * pk.step < DV;
@@ -574,18 +591,18 @@ k_norm_fwd(NormFwd a, RowMap m) {
       mix_pack<T, V>(raw[k], pre, v[k]);
       if (a.sum_out && ok) PackIO<T, V>::store_round(so + k * stride, v[k]);
     } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e) v[k][e] = raw_get<V>(raw[k][0], e);
+      unpack<T, V>(raw[k][0], v[k]);
       if constexpr (DROP) drop_apply<V>(a.drop, bits[k], v[k]);
       if (a.res) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(raw[k][1], e);
+        float u[V];
+        unpack<T, V>(raw[k][1], u);
+        pack_add<V>(v[k], u);
       }
       if (a.sum_out && ok) PackIO<T, V>::store(so + k * stride, v[k]);
     }
     norm_gather<V, OUT>(v[k], w[k], ss, mx);
   }
-  norm_emit<T, V, NP, OUT>(a, m, pk, sm, sub, t, DV, row, at, v, w, ss, mx);
+  norm_emit<T, V, NP, OUT>(a, m, pk, sm, sub, t, DV, row, at, v, w, total(ss), mx);
 }
 
 // Many rows and more to do per pack than to add, norm and store it (8-bit output, dropout): persistent CTAs that keep the
@@ -659,7 +676,8 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
     if constexpr (DROP)   // while the row is on its way
       drop_row_bits<V, NP>(seed, dcol, drop_row(a.drop, seed, row), pk, nullptr, bits);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
-    float v[NP][V], ss = 0.f, mx = 0.f;
+    float v[NP][V], mx = 0.f;
+    Sum2 ss{0};
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
 #pragma unroll
@@ -672,21 +690,19 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
           mix_pack<T, V>(x, pre, v[k]);
           if (a.sum_out) PackIO<T, V>::store_round((T*)a.sum_out + at + k * stride, v[k]);
         } else {
-          const RawPack<T, V> x = slot(stage, k, 0);
-#pragma unroll
-          for (int e = 0; e < V; ++e) v[k][e] = raw_get<V>(x, e);
+          unpack<T, V>(slot(stage, k, 0), v[k]);
           if constexpr (DROP) drop_apply<V>(a.drop, bits[k], v[k]);
           if (a.res) {
-            const RawPack<T, V> r = slot(stage, k, 1);
-#pragma unroll
-            for (int e = 0; e < V; ++e) v[k][e] += raw_get<V>(r, e);
+            float u[V];
+            unpack<T, V>(slot(stage, k, 1), u);
+            pack_add<V>(v[k], u);
           }
           if (a.sum_out) PackIO<T, V>::store((T*)a.sum_out + at + k * stride, v[k]);
         }
         norm_gather<V, OUT>(v[k], w[k], ss, mx);
       }
     }
-    norm_emit<T, V, NP, OUT>(a, m, pk, sm[stage], sub, t, DV, row, at, v, w, ss, mx);
+    norm_emit<T, V, NP, OUT>(a, m, pk, sm[stage], sub, t, DV, row, at, v, w, total(ss), mx);
     stage ^= 1;   // the next row's sums go to the other half of sm: nobody can still be reading it
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -791,7 +807,8 @@ k_norm_bwd(NormBwd a, RowMap m) {
     return r;
   };
 
-  float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  float pre[4] = {0.f, 0.f, 0.f, 0.f};
+  Sum2 acc[4] = {};
   uint32_t pre_of = 0xffffffffu;
   int parity = 0, stage = 0;
   float ahead[DEPTH > 1 ? DEPTH - 1 : 1];   // rstd of the rows on the way
@@ -857,7 +874,8 @@ k_norm_bwd(NormBwd a, RowMap m) {
         for (int n = 0; n < 4; ++n) pre[n] = __ldg(a.hpre + (int64_t)(q.item / chunks) * 4 + n);
       }
     }
-    float s[NP][V], h[NP][V], c = 0.f, unused = 0.f;
+    float s[NP][V], h[NP][V], unused = 0.f;
+    Sum2 c2{0};
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
 #pragma unroll
@@ -872,26 +890,26 @@ k_norm_bwd(NormBwd a, RowMap m) {
           for (int n = 0; n < 4; ++n) x[n] = pack(k, 1 + n);
           mix_pack<T, V>(x, pre, s[k]);
         } else {
-          const RawPack<T, V> x = pack(k, 1);
-#pragma unroll
-          for (int e = 0; e < V; ++e) s[k][e] = raw_get<V>(x, e);
+          unpack<T, V>(pack(k, 1), s[k]);
           if constexpr (DROP) drop_apply<V>(a.drop, bits[k], s[k]);
           if (a.res) {
-            const RawPack<T, V> r = pack(k, 2);
-#pragma unroll
-            for (int e = 0; e < V; ++e) s[k][e] += raw_get<V>(r, e);
+            float u[V];
+            unpack<T, V>(pack(k, 2), u);
+            pack_add<V>(s[k], u);
           }
         }
+        unpack<T, V>(dy, h[k]);
+        pack_scale<V>(h[k], rstd);
+        if (kSelect && !(live && own[k])) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          float g = raw_get<V>(dy, e) * rstd;
-          if (kSelect && !(live && own[k])) g = s[k][e] = 0.f;
-          h[k][e] = g * w[k][e];
-          c = fmaf(h[k][e], s[k][e], c);
-          dw[k][e] = fmaf(g, s[k][e], dw[k][e]);
+          for (int e = 0; e < V; ++e) h[k][e] = s[k][e] = 0.f;
         }
+        pack_fma<V>(dw[k], h[k], s[k]);
+        pack_mul<V>(h[k], w[k]);
+        pack_dot<V>(c2, h[k], s[k]);
       }
     }
+    float c = total(c2);
     row_sum_max<false>(c, unused, sm[parity], m, sub);
     parity ^= 1;   // the next row's sums go to the other half: nobody can still be reading it
     const float kk = c * rstd * rstd * a.inv_D;   // c holds one rstd already
@@ -900,25 +918,25 @@ k_norm_bwd(NormBwd a, RowMap m) {
       if (live && own[k]) {
         float g[V];
 #pragma unroll
-        for (int e = 0; e < V; ++e) g[e] = fmaf(-kk, s[k][e], h[k][e]);
+        for (int e = 0; e < V; ++e) g[e] = -kk;
+        pack_mul_add<V>(g, s[k], h[k]);
         if constexpr (SRC == Src::Mix) {
           T* o = (T*)a.dx + row * 4 * D + pk.first * V + k * stride;
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
-            const RawPack<T, V> x = pack(k, 1 + n);
-            float u[V];
+            float x[V], u[V];
+            unpack<T, V>(pack(k, 1 + n), x);
+            pack_dot<V>(acc[n], g, x);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-              acc[n] = fmaf(g[e], raw_get<V>(x, e), acc[n]);
-              u[e] = pre[n] * g[e];
-            }
+            for (int e = 0; e < V; ++e) u[e] = g[e];
+            pack_scale<V>(u, pre[n]);
             PackIO<T, V>::store(o + n * D, u);
           }
         } else {
           if (a.dsum) {
-            const RawPack<T, V> ds = pack(k, 3);
-#pragma unroll
-            for (int e = 0; e < V; ++e) g[e] += raw_get<V>(ds, e);
+            float u[V];
+            unpack<T, V>(pack(k, 3), u);
+            pack_add<V>(g, u);
           }
           if constexpr (DROP) {
             if (a.dres) PackIO<T, V>::store((T*)a.dres + row * D + pk.first * V + k * stride, g);
@@ -931,9 +949,10 @@ k_norm_bwd(NormBwd a, RowMap m) {
     if constexpr (SRC == Src::Mix) {
       if (q2.item != q.item) {
         __syncthreads();   // the previous item's readers of red are done
-        block_reduce_store<4>(acc, a.dpre_part + (int64_t)q.item * 4, red);
+        float sums[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) acc[n] = 0.f;
+        for (int n = 0; n < 4; ++n) sums[n] = total(acc[n]), acc[n].s = 0;
+        block_reduce_store<4>(sums, a.dpre_part + (int64_t)q.item * 4, red);
       }
     }
     q = q2;
