@@ -239,7 +239,7 @@ int mhc_add_residual_dropout_bwd(const void* dH_new, const void* branch_output, 
  * s = x (through the dropout above where drop_threshold != 0) + residual (may be NULL);
  * rstd = 1 / sqrt(mean_d s^2 + eps);  y = s * rstd * weight.
  * weight: [D] fp32 or of the activation type (weight_dtype), or NULL for ones.  sum_out (s rounded to
- * the activation type; what the backward reads) and rstd [rows] fp32 may be NULL.  s is normalised
+ * the activation type) and rstd [rows] fp32 (what the backward reads) may be NULL.  s is normalised
  * as computed, before that rounding.  The reference leaves norms to the caller. */
 int mhc_add_rms_norm_fwd(const void* x, const void* residual, const void* weight, int weight_dtype,
                          const int64_t* rng, int drop_threshold, int64_t row_offset, void* sum_out, void* y,

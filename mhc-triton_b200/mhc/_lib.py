@@ -233,7 +233,12 @@ def tickets(like: torch.Tensor, n: int):
 def eager_tickets(like: torch.Tensor, n: int):
     """`tickets`, but none while a CUDA graph is captured: graphs captured on one stream would share its counters and
     could be replayed at the same time."""
-    return None if torch.cuda.is_current_stream_capturing() else tickets(like, n)
+    if like.get_device() == torch._C._cuda_getDevice():
+        capturing = torch.cuda.is_current_stream_capturing()
+    else:
+        with torch.cuda.device(like.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+    return None if capturing else tickets(like, n)
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

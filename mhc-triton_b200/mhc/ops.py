@@ -10,6 +10,7 @@ the single write of dH instead of a separate read-modify-write pass.
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._backward import (add_residual_backward, add_residual_dropout_backward, fused_dynamic_weights_backward,
@@ -231,6 +232,13 @@ class _HyperConnectionMix(torch.autograd.Function):
                 galpha[2:3].reshape_as(alpha_res).to(alpha_res.dtype)) + (None,) * 8 + (d_norm_weight, None)
 
 
+def _first_order(backward):
+    """once_differentiable (an error where a gradient's gradient is asked for) at no cost where none can be: grad mode
+    is on in a backward only with create_graph=True."""
+    checked = once_differentiable(backward)
+    return lambda ctx, *grads: checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+
 class _AddResidualDropout(torch.autograd.Function):
     """_FusedAddResidual (H_res None) and _AddResidualFromState (first input: the storage-less stand-in) with the
     branch output passed through the counter-based dropout.  The mask is recomputed in the backward from `rng`."""
@@ -247,6 +255,7 @@ class _AddResidualDropout(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_first_order
     def backward(ctx, grad_H_new, _unused=None):
         if grad_H_new is None:
             return (None,) * 9
@@ -254,13 +263,6 @@ class _AddResidualDropout(torch.autograd.Function):
         dH_residual, d_bo, dH_post = add_residual_dropout_backward(grad_H_new, branch_output, H_post, rng,
                                                                    ctx.threshold, ctx.row_offset)
         return (dH_residual, None, None, d_bo.to(branch_output.dtype), dH_post.to(H_post.dtype)) + (None,) * 4
-
-
-def _first_order(backward):
-    """once_differentiable (an error where a gradient's gradient is asked for) at no cost where none can be: grad mode
-    is on in a backward only with create_graph=True."""
-    checked = once_differentiable(backward)
-    return lambda ctx, *grads: checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
 
 class _CounterDropout(torch.autograd.Function):
@@ -441,11 +443,13 @@ def hyper_connection_mix(H, H_pre_base, H_post_base, H_res_base, phi, alpha_pre,
 
 
 def _records(*tensors) -> bool:
-    """Whether autograd would record an operation on these."""
+    """Whether autograd would record an operation on these, in reverse or (to refuse it) in forward mode."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
+    if forward_ad._current_level >= 0:
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
     return False
 
 

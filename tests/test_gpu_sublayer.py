@@ -789,6 +789,33 @@ def test_refusals_on_the_gpu():
         g.sum().backward()           # no second derivative
 
 
+def test_derivatives_that_do_not_exist_are_refused():
+    """Second derivatives and forward-mode tangents raise instead of leaving terms out."""
+    import mhc
+    from torch.autograd import forward_ad
+    B, S, D = 2, 3, 64
+    H, bo = torch.randn(B, S, 4, D, device="cuda"), torch.randn(B, S, D, device="cuda")
+    Hp, w = torch.rand(B, 4, device="cuda"), torch.ones(D, device="cuda")
+    leaf = bo.clone().requires_grad_(True)
+    out = mhc.fused_add_residual(H, leaf, Hp, dropout_p=0.25, rng=(1, 2))
+    (g,) = torch.autograd.grad((out * out).sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    calls = [lambda b, h: mhc.counter_dropout(b, 0.25, rng=(1, 2)), lambda b, h: mhc.fused_add_rms_norm(b, None, w),
+             lambda b, h: mhc.fused_stream_norm(h, Hp, w), lambda b, h: mhc.fused_add_rms_norm_quant(b, None, w),
+             lambda b, h: mhc.fused_stream_norm_quant(h, Hp, w),
+             lambda b, h: mhc.fused_add_residual(h, b, Hp, dropout_p=0.25, rng=(1, 2))]
+    for call in calls:
+        with torch.no_grad():
+            call(bo, H)
+        with forward_ad.dual_level():
+            call(bo, H)              # nothing carries a tangent
+            dual_b = forward_ad.make_dual(bo, torch.ones_like(bo))
+            dual_h = forward_ad.make_dual(H, torch.ones_like(H))
+            with pytest.raises(RuntimeError):
+                call(dual_b, dual_h)
+
+
 def test_many_rows_past_32_bit_offsets():
     """A tensor of more than 2^31 elements: the last rows must be the last rows."""
     import mhc
