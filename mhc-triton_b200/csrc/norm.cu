@@ -253,13 +253,13 @@ k_norm_any_fwd(NormFwd a) {
 }
 
 // Persistent CTAs of 256 threads: CTA i takes items i, i + grid, ...  An item is a row (Add), or a share of the tokens of
-// one batch element (Mix), whose dH_pre it sums.  dweight's partial sums live in the CTA's own row of dw_part.
+// one batch element (Mix), whose dH_pre it sums (block_store_f64).  dweight's partial sums live in the CTA's own row of dw_part.
 template <typename T, Src SRC, bool DROP>
 __global__ void __launch_bounds__(256)
 k_norm_any_bwd(NormBwd a) {
   pdl_prologue();
   __shared__ float sm[64];
-  __shared__ float red[8 * 4];
+  __shared__ double red[8 * 4];
   const int64_t D = a.D;
   DropSeed seed{};
   if constexpr (DROP) seed = drop_seed(a.drop);
@@ -268,7 +268,8 @@ k_norm_any_bwd(NormBwd a) {
     for (int64_t d = threadIdx.x; d < D; d += 256) dw[d] = 0.f;
   for (int64_t it = blockIdx.x; it < a.items; it += gridDim.x) {
     int64_t r0 = it, r1 = it + 1;   // RowMap of this kernel: one row at a time
-    float pre[4] = {0.f, 0.f, 0.f, 0.f}, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    float pre[4] = {0.f, 0.f, 0.f, 0.f};
+    double dpre[4] = {0.0, 0.0, 0.0, 0.0};
     if constexpr (SRC == Src::Mix) {
       const int64_t b = it / a.chunks;
       r0 = b * a.S + it % a.chunks;
@@ -290,6 +291,7 @@ k_norm_any_bwd(NormBwd a) {
       __syncthreads();  // the previous row's readers of sm are done
       block_sum_max<false>(c, unused, sm);
       const float k = c * rstd * rstd * rstd * a.inv_D;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (int64_t d = threadIdx.x; d < D; d += 256) {
         const float dy = to_f32(__ldg((const T*)a.dy + row * D + d));
         float g[1] = {rstd * (dy * load_w<T>(a.weight, a.w_f32, d)) - s_at(d) * k};
@@ -310,10 +312,14 @@ k_norm_any_bwd(NormBwd a) {
           ((T*)a.dx)[row * D + d] = from_f32<T>(g[0]);
         }
       }
+      if constexpr (SRC == Src::Mix) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) dpre[n] += (double)acc[n];
+      }
     }
     if constexpr (SRC == Src::Mix) {
       __syncthreads();
-      block_reduce_store<4>(acc, a.dpre_part + it * 4, red);
+      block_store_f64(dpre, a.dpre_part + it * 4, red);
     }
   }
 }
@@ -721,7 +727,7 @@ __global__ void __launch_bounds__(THREADS)
 k_norm_bwd(NormBwd a, RowMap m) {
   extern __shared__ __align__(16) uint4 ring[];   // [DEPTH][NP][NS][threads]
   __shared__ float sm[2][64];
-  __shared__ float red[32 * 4];
+  __shared__ double red[SRC == Src::Mix ? 32 * 4 : 1];
   __shared__ uint4 exchange[DROP && V == 1 ? 1024 : 1];
   pdl_prologue();
   constexpr int NS = SRC == Src::Mix ? 5 : 4;   // Mix: dy, H[0..3]; Add: dy, x, residual, dsum
@@ -808,7 +814,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
   };
 
   float pre[4] = {0.f, 0.f, 0.f, 0.f};
-  Sum2 acc[4] = {};
+  double dpre[4] = {0.0, 0.0, 0.0, 0.0};
   uint32_t pre_of = 0xffffffffu;
   int parity = 0, stage = 0;
   float ahead[DEPTH > 1 ? DEPTH - 1 : 1];   // rstd of the rows on the way
@@ -913,6 +919,7 @@ k_norm_bwd(NormBwd a, RowMap m) {
     row_sum_max<false>(c, unused, sm[parity], m, sub);
     parity ^= 1;   // the next row's sums go to the other half: nobody can still be reading it
     const float kk = c * rstd * rstd * a.inv_D;   // c holds one rstd already
+    Sum2 acc[4] = {};
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       if (live && own[k]) {
@@ -947,12 +954,13 @@ k_norm_bwd(NormBwd a, RowMap m) {
       }
     }
     if constexpr (SRC == Src::Mix) {
+#pragma unroll
+      for (int n = 0; n < 4; ++n) dpre[n] += (double)total(acc[n]);
       if (q2.item != q.item) {
         __syncthreads();   // the previous item's readers of red are done
-        float sums[4];
+        block_store_f64(dpre, a.dpre_part + (int64_t)q.item * 4, red);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) sums[n] = total(acc[n]), acc[n].s = 0;
-        block_reduce_store<4>(sums, a.dpre_part + (int64_t)q.item * 4, red);
+        for (int n = 0; n < 4; ++n) dpre[n] = 0.0;
       }
     }
     q = q2;

@@ -553,11 +553,13 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             unpack<T, V>(u.p[n], x);
+            float sum = DROP ? 0.f : acc[n];   // DROP walks more tokens: a pack's sum by itself halves dH_post's error
 #pragma unroll
             for (int e = 0; e < V; ++e) {
               z[e] = fmaf(p[n], x[e], z[e]);
-              acc[n] = fmaf(x[e], y[e], acc[n]);
+              sum = fmaf(x[e], y[e], sum);
             }
+            acc[n] = DROP ? acc[n] + sum : sum;
           }
           if constexpr (DROP) drop_apply<V>(drop, bits, z);
           PackIO<T, V>::store(dbo + (tok + s) * D + c0, z);
@@ -572,7 +574,12 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
     else
       for_tokens<MHC_ADDBWD_PIPE != 0, B5>(it.s0 + it.sub, it.s1, g.sub, load, compute);
   }
-  block_reduce_store<4>(acc, part + (it.b * geo_slots_dev(g) + it.slot) * 4, red);
+  if constexpr (DROP) {
+    double sums[4] = {acc[0], acc[1], acc[2], acc[3]};
+    block_store_f64(sums, part + (it.b * geo_slots_dev(g) + it.slot) * 4, reinterpret_cast<double*>(red));
+  } else {
+    block_reduce_store<4>(acc, part + (it.b * geo_slots_dev(g) + it.slot) * 4, red);
+  }
   if (!tickets) return;
   const int64_t slots = geo_slots_dev(g);
   if (cta_arrives_last(tickets + it.b, (int)slots))
