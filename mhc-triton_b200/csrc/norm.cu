@@ -614,7 +614,7 @@ k_norm_fwd(NormFwd a, RowMap m) {
 // Many rows and more to do per pack than to add, norm and store it (8-bit output, dropout): persistent CTAs that keep the
 // weight and the columns' part of the generator in registers, with the next row's packs on the way by cp.async into slots of
 // shared memory that only the thread itself reads.  The one-shot form is bound by instructions there: 16384 x 7168 bf16 to
-// e4m3 with a scale per 32 columns 170 us against 132 (6.2 TB/s), 8192 x 7168 with dropout 90 against 82.
+// e4m3 with a scale per 32 columns 170 us against 132-137 (6.0-6.2 TB/s), 8192 x 7168 with dropout 90 against 81.
 template <typename T, int V, int NP, Src SRC, bool DROP, Out OUT>
 __global__ void __launch_bounds__(512, 2)
 k_norm_fwd_ring(NormFwd a, RowMap m) {

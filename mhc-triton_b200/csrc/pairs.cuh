@@ -82,7 +82,9 @@ template <int V> __device__ __forceinline__ void pack_mul_add(float (&a)[V], con
 struct Sum2 { uint64_t s; };
 template <int V> __device__ __forceinline__ void pack_dot(Sum2& sum, const float (&a)[V], const float (&b)[V]) {
   if constexpr (V == 1) {
-    sum.s = fma2(pair(a[0], 0.f), pair(b[0], 0.f), sum.s);
+    float lo, hi;
+    unpair(sum.s, lo, hi);
+    sum.s = pair(fmaf(a[0], b[0], lo), hi);
   } else {
 #pragma unroll
     for (int e = 0; e < V; e += 2) sum.s = fma2(pair(a[e], a[e + 1]), pair(b[e], b[e + 1]), sum.s);

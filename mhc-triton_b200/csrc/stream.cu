@@ -553,7 +553,7 @@ k_add_residual_bwd(const T* __restrict__ G, const T* __restrict__ bo, const floa
 #pragma unroll
           for (int n = 0; n < 4; ++n) {
             unpack<T, V>(u.p[n], x);
-            float sum = DROP ? 0.f : acc[n];   // DROP walks more tokens: a pack's sum by itself halves dH_post's error
+            float sum = DROP ? 0.f : acc[n];   // DROP walks more tokens: a pack is summed by itself, for dH_post's accuracy
 #pragma unroll
             for (int e = 0; e < V; ++e) {
               z[e] = fmaf(p[n], x[e], z[e]);
