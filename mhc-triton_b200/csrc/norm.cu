@@ -568,7 +568,7 @@ k_norm_fwd(NormFwd a, RowMap m) {
   float pre[4] = {0.f, 0.f, 0.f, 0.f};
   if constexpr (SRC == Src::Mix) {
     if (DV) {
-      const float* h = a.hpre + (uint32_t)row / (uint32_t)a.S * 4;   // at most 2^31 rows
+      const float* h = a.hpre + (int64_t)((uint32_t)row / (uint32_t)a.S) * 4;   // at most 2^31 rows, four weights each
 #pragma unroll
       for (int n = 0; n < 4; ++n) pre[n] = __ldg(h + n);
     }
@@ -673,7 +673,7 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
     float pre[4] = {0.f, 0.f, 0.f, 0.f};
     if constexpr (SRC == Src::Mix) {
       if (DV) {
-        const float* h = a.hpre + row / (uint32_t)a.S * 4;
+        const float* h = a.hpre + (int64_t)(row / (uint32_t)a.S) * 4;
 #pragma unroll
         for (int n = 0; n < 4; ++n) pre[n] = __ldg(h + n);
       }
