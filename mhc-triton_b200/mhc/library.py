@@ -293,16 +293,15 @@ def _rms_norm_bwd(dy: Tensor, dsum: Optional[Tensor], x: Tensor, residual: Optio
                   row_offset: int) -> Tuple[Tensor, Tensor, Tensor]:
     dx, dres, dw = B.rms_norm_backward(dy, dsum, x, residual, rstd, weight, rng, threshold, row_offset,
                                        want_dresidual=residual is not None, want_dweight=weight is not None)
-    none = x.new_empty(0)       # absent outputs: no residual's own gradient without dropout, no weight
-    return dx, (dres if threshold and residual is not None else none), (none if dw is None else dw)
+    # absent outputs (no residual's own gradient without dropout, no weight): a tensor each, outputs may not alias
+    return (dx, dres if threshold and residual is not None else x.new_empty(0), x.new_empty(0) if dw is None else dw)
 
 
 @_rms_norm_bwd.register_fake
 def _(dy, dsum, x, residual, rstd, weight, rng, threshold, row_offset):
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    none = x.new_empty(0)
-    return (dx, torch.empty_like(dx) if threshold and residual is not None else none,
-            none if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format))
+    return (dx, torch.empty_like(dx) if threshold and residual is not None else x.new_empty(0),
+            x.new_empty(0) if weight is None else torch.empty_like(weight, memory_format=torch.contiguous_format))
 
 
 def _norm_setup(ctx, inputs, output):
