@@ -7,11 +7,11 @@ stream mix in one autograd Function, so that the gradient of the pooled state is
 the single write of dH instead of a separate read-modify-write pass.
 """
 
+import functools
 from typing import Optional, Tuple
 
 import torch
 from torch.autograd import forward_ad
-from torch.autograd.function import once_differentiable
 
 from ._backward import (add_residual_backward, add_residual_dropout_backward, fused_dynamic_weights_backward,
                         hc_mix_backward, rms_norm_backward, sinkhorn_backward, stream_mix_backward,
@@ -232,11 +232,40 @@ class _HyperConnectionMix(torch.autograd.Function):
                 galpha[2:3].reshape_as(alpha_res).to(alpha_res.dtype)) + (None,) * 8 + (d_norm_weight, None)
 
 
-def _first_order(backward):
-    """once_differentiable (an error where a gradient's gradient is asked for) at no cost where none can be: grad mode
-    is on in a backward only with create_graph=True."""
-    checked = once_differentiable(backward)
-    return lambda ctx, *grads: checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+class _NoSecondDerivative(torch.autograd.Function):
+    """Hands gradients on; differentiating them is an error.  `anchor` requires a gradient, so the result always does."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(g.view_as(g) for g in grads)    # one tensor may stand for two inputs' gradients
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("mhc: this operator has no second derivative")
+
+
+def _first_order(depends):
+    """Decorates the `backward` of a node whose kernels' results cannot be differentiated.  Under create_graph=True (grad mode
+    is on in a backward only then) they come out such that differentiating them is an error, where the upstream gradients
+    are differentiated or the gradients depend on the node's own differentiated inputs (`depends(ctx, *grads)`).  Elsewhere
+    they are constants; an upstream gradient that is handed through stays what it is."""
+    return lambda backward: functools.partial(_run_first_order, backward, depends)
+
+
+def _run_first_order(backward, depends, ctx, *grads):
+    if not torch.is_grad_enabled():
+        return backward(ctx, *grads)
+    with torch.no_grad():
+        out = backward(ctx, *grads)
+    given = [g for g in grads if g is not None]
+    if not depends(ctx, *grads) and not any(g.requires_grad for g in given):
+        return out
+    which = [i for i, o in enumerate(out) if o is not None and not any(o is g for g in given)]
+    if not which:
+        return out
+    anchor = torch.empty(0, device=out[which[0]].device, requires_grad=True)
+    marked = dict(zip(which, _NoSecondDerivative.apply(anchor, *[out[i] for i in which])))
+    return tuple(marked.get(i, o) for i, o in enumerate(out))
 
 
 class _AddResidualDropout(torch.autograd.Function):
@@ -255,7 +284,7 @@ class _AddResidualDropout(torch.autograd.Function):
         return out
 
     @staticmethod
-    @_first_order
+    @_first_order(lambda ctx, *_: ctx.needs_input_grad[3] and ctx.needs_input_grad[4])    # each depends on the other input
     def backward(ctx, grad_H_new, _unused=None):
         if grad_H_new is None:
             return (None,) * 9
@@ -273,7 +302,7 @@ class _CounterDropout(torch.autograd.Function):
         return counter_dropout_forward(x, rng, threshold, row_offset)
 
     @staticmethod
-    @_first_order
+    @_first_order(lambda ctx, *_: False)    # linear
     def backward(ctx, grad):
         (rng,) = ctx.saved_tensors
         return counter_dropout_forward(grad, rng, ctx.threshold, ctx.row_offset), None, None, None
@@ -291,7 +320,8 @@ class _AddRmsNorm(torch.autograd.Function):
         return (y, s) if residual is not None or threshold else y
 
     @staticmethod
-    @_first_order
+    # s is linear in x and the residual, and the weight's gradient does not depend on the weight
+    @_first_order(lambda ctx, dy, ds=None: dy is not None and any(ctx.needs_input_grad[:2]))
     def backward(ctx, dy, ds=None):
         if dy is None and ds is None:
             return (None,) * 7
@@ -314,7 +344,7 @@ class _FusedStreamNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @_first_order
+    @_first_order(lambda ctx, *_: any(ctx.needs_input_grad[:2]))
     def backward(ctx, dy):
         H, H_pre, weight, rstd = ctx.saved_tensors
         dH, dH_pre, dw = stream_norm_backward(dy, H, H_pre, rstd, weight, want_dweight=ctx.needs_input_grad[2])
