@@ -160,6 +160,43 @@ class _SequenceMeanPool(torch.autograd.Function):
         return (gx.reshape(B, 1, n, D) / S).to(ctx.dtype).expand(B, S, n, D)
 
 
+class _NoSecondDerivative(torch.autograd.Function):
+    """Hands gradients on; differentiating them is an error.  `anchor` requires a gradient, so the result always does."""
+
+    @staticmethod
+    def forward(ctx, anchor, *grads):
+        return tuple(g.view_as(g) for g in grads)    # one tensor may stand for two inputs' gradients
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("mhc: this operator has no second derivative")
+
+
+def _first_order(depends, applies=lambda ctx: True):
+    """Decorates the `backward` of a node whose kernels' results cannot be differentiated.  Under create_graph=True (grad mode
+    is on in a backward only then) they come out such that differentiating them is an error, where the upstream gradients
+    are differentiated or the gradients depend on the node's own differentiated inputs (`depends(ctx, *grads)`).  Elsewhere
+    they are constants; an upstream gradient that is handed through stays what it is.  Nodes for which `applies` is false run
+    `backward` as it is."""
+    return lambda backward: functools.partial(_run_first_order, backward, depends, applies)
+
+
+def _run_first_order(backward, depends, applies, ctx, *grads):
+    if not (torch.is_grad_enabled() and applies(ctx)):
+        return backward(ctx, *grads)
+    with torch.no_grad():
+        out = backward(ctx, *grads)
+    given = [g for g in grads if g is not None]
+    if not depends(ctx, *grads) and not any(g.requires_grad for g in given):
+        return out
+    which = [i for i, o in enumerate(out) if o is not None and not any(o is g for g in given)]
+    if not which:
+        return out
+    anchor = torch.empty(0, device=out[which[0]].device, requires_grad=True)
+    marked = dict(zip(which, _NoSecondDerivative.apply(anchor, *[out[i] for i in which])))
+    return tuple(marked.get(i, o) for i, o in enumerate(out))
+
+
 class _HyperConnectionMix(torch.autograd.Function):
     """Mean-pool + dynamic weights + stream mix as one autograd node.
 
@@ -202,7 +239,10 @@ class _HyperConnectionMix(torch.autograd.Function):
         ctx.set_materialize_grads(False)   # no zero-filled gradients for outputs nobody used
         return branch_input, H_residual, H_post, H_pre, H_res
 
+    # With the norm no term may be left out (its weight's gradient alone does not depend on the weight); without it the
+    # gradients have always come back as constants.
     @staticmethod
+    @_first_order(lambda ctx, *_: any(ctx.needs_input_grad[:8]), applies=lambda ctx: ctx.has_norm)
     def backward(ctx, d_branch_input, dH_residual, dH_post, _unused_pre, _unused_res):
         (H, x, phi, pre_b, post_b, res_b, alpha_pre, alpha_post, alpha_res, saved, H_pre, H_res) = ctx.saved_tensors[:12]
         B, S, _, D = H.shape
@@ -230,42 +270,6 @@ class _HyperConnectionMix(torch.autograd.Function):
                 galpha[0:1].reshape_as(alpha_pre).to(alpha_pre.dtype),
                 galpha[1:2].reshape_as(alpha_post).to(alpha_post.dtype),
                 galpha[2:3].reshape_as(alpha_res).to(alpha_res.dtype)) + (None,) * 8 + (d_norm_weight, None)
-
-
-class _NoSecondDerivative(torch.autograd.Function):
-    """Hands gradients on; differentiating them is an error.  `anchor` requires a gradient, so the result always does."""
-
-    @staticmethod
-    def forward(ctx, anchor, *grads):
-        return tuple(g.view_as(g) for g in grads)    # one tensor may stand for two inputs' gradients
-
-    @staticmethod
-    def backward(ctx, *grads):
-        raise RuntimeError("mhc: this operator has no second derivative")
-
-
-def _first_order(depends):
-    """Decorates the `backward` of a node whose kernels' results cannot be differentiated.  Under create_graph=True (grad mode
-    is on in a backward only then) they come out such that differentiating them is an error, where the upstream gradients
-    are differentiated or the gradients depend on the node's own differentiated inputs (`depends(ctx, *grads)`).  Elsewhere
-    they are constants; an upstream gradient that is handed through stays what it is."""
-    return lambda backward: functools.partial(_run_first_order, backward, depends)
-
-
-def _run_first_order(backward, depends, ctx, *grads):
-    if not torch.is_grad_enabled():
-        return backward(ctx, *grads)
-    with torch.no_grad():
-        out = backward(ctx, *grads)
-    given = [g for g in grads if g is not None]
-    if not depends(ctx, *grads) and not any(g.requires_grad for g in given):
-        return out
-    which = [i for i, o in enumerate(out) if o is not None and not any(o is g for g in given)]
-    if not which:
-        return out
-    anchor = torch.empty(0, device=out[which[0]].device, requires_grad=True)
-    marked = dict(zip(which, _NoSecondDerivative.apply(anchor, *[out[i] for i in which])))
-    return tuple(marked.get(i, o) for i, o in enumerate(out))
 
 
 class _AddResidualDropout(torch.autograd.Function):

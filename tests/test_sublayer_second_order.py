@@ -120,3 +120,57 @@ def test_gradients_without_a_second_derivative_around_stub_kernels(monkeypatch):
 @pytest.mark.gpu
 def test_gradients_without_a_second_derivative():
     _nothing_left_out("cuda")
+
+
+# -------------------------------------------------------------------------------------------------- the layer's own node
+def _layer(device, norm):
+    import mhc
+    torch.manual_seed(0)
+    hc = mhc.HyperConnection(dim=64).to(device)
+    H = torch.randn(2, 5, 4, 64).to(device).requires_grad_(True)
+    w = torch.rand(64).to(device).add_(0.5).requires_grad_(True)
+    y, add = hc(H, w) if norm else hc(H)
+    return y, add, H, w
+
+
+def _layer_with_norm(device):
+    y, add, H, w = _layer(device, True)
+    _refused(_first(y, [H, w]), [H, w])
+    y, add, H, w = _layer(device, True)
+    _refused(_first(y.square().sum(), [H, w]), [H, w])
+    y, add, H, w = _layer(device, True)
+    _refused(_first(add(torch.tanh(y), dropout_p=0.25, rng=torch.tensor([1, 2], device=device)), [H, w]), [H, w])
+    for with_graph in (False, True):
+        y, add, H, w = _layer(device, True)
+        a = torch.autograd.grad(y.sum(), [H, w], create_graph=with_graph)
+        y, add, H, w = _layer(device, True)
+        for p, q in zip(a, torch.autograd.grad(y.sum(), [H, w])):
+            assert torch.equal(p.detach(), q)
+
+
+def test_layer_with_norm_around_stub_kernels(monkeypatch):
+    _stub(monkeypatch)
+    like = torch.ones_like
+
+    def mix_norm(H, *a, **k):
+        B, S, _, D = H.shape
+        return (H.sum(2), H.sum(2), H.new_ones(B * S), H.new_ones(B, 4), H.new_ones(B, 4), H.new_ones(B, 4, 4),
+                H.new_ones(B, 4 * D), H.new_ones(B, 32))
+
+    monkeypatch.setattr(ops, "hc_mix_norm_forward", mix_norm)
+    monkeypatch.setattr(ops, "hc_mix_backward", lambda dbi, dHr, dp, H, x, phi, *a, **k: (
+        like(H), like(phi), phi.new_ones(24), phi.new_ones(3)))
+    _layer_with_norm("cpu")
+
+
+@pytest.mark.gpu
+def test_layer_with_norm():
+    _layer_with_norm("cuda")
+
+
+@pytest.mark.gpu
+def test_layer_without_norm_is_as_it_was():
+    y, add, H, w = _layer("cuda", False)
+    (g,) = _first(y, [H])
+    (g.square().sum() + H.square().sum()).backward()
+    assert torch.equal(H.grad, 2 * H.detach())
