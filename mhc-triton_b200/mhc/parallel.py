@@ -256,6 +256,12 @@ def _group_size(group) -> int:
     return dist.get_world_size(group)
 
 
+def _group_rank(group) -> int:
+    if not (dist.is_available() and dist.is_initialized()):
+        return 0
+    return dist.get_rank(group)
+
+
 class SequenceShardedHyperConnection(torch.nn.Module):
     """Wraps a fused dynamic HyperConnection for inputs sharded along the sequence axis.
 
@@ -283,8 +289,15 @@ class SequenceShardedHyperConnection(torch.nn.Module):
         if norm_weight is not None or norm_eps is not None:
             branch_input = fused_add_rms_norm(branch_input, None, norm_weight, 1e-6 if norm_eps is None else norm_eps)[0]
 
-        def add_residual(branch_output: torch.Tensor, dropout_p: float = 0.0, rng=None, row_offset: int = 0) -> torch.Tensor:
-            """The dropout counts this rank's own tokens as rows: pass a different rng, or another row_offset, per rank."""
+        def add_residual(branch_output: torch.Tensor, dropout_p: float = 0.0, rng=None,
+                         row_offset: Optional[int] = None) -> torch.Tensor:
+            """Dropout counts this rank's token s of batch element b as row row_offset + b * S_local + s.  By default every rank
+            has rows of its own, also where all of them draw the same rng: row_offset = rank * batch * S_local (with one
+            sequence that is the mask of the whole tensor), or rank * batch * total_len where total_len is given, since
+            shards may then be of different lengths.  A row_offset that is given is taken as it is."""
+            if row_offset is None:
+                tokens = H.shape[1] if self.total_len is None else self.total_len
+                row_offset = _group_rank(self.group) * H.shape[0] * tokens
             return add_residual_from_state(stand_in, H, H_res, branch_output, H_post, False, dropout_p, rng, row_offset)
 
         return branch_input, add_residual
