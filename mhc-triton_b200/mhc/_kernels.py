@@ -221,6 +221,14 @@ def dropout_rng(rng, like: torch.Tensor) -> torch.Tensor:
     return torch.tensor([v - (1 << 64) if v >> 63 else v for v in (seed, offset)], device=like.device, dtype=torch.int64)
 
 
+def row_number(row_offset) -> int:
+    """row_offset as an int that the library can be given (it refuses what is not in [0, 2^32 - rows])."""
+    row_offset = int(row_offset)
+    if not -(1 << 63) <= row_offset < 1 << 63:
+        raise ValueError(f"row_offset must be in [0, 2^32), got {row_offset}")
+    return row_offset
+
+
 def _rows_of(t: torch.Tensor) -> Tuple[int, int]:
     """(rows, columns) of a tensor whose last axis are the columns."""
     D = t.shape[-1]

@@ -19,7 +19,7 @@ from ._backward import (add_residual_backward, add_residual_dropout_backward, fu
 from ._kernels import (add_residual_dropout_forward, add_residual_forward, add_residual_mix_forward,
                        add_rms_norm_forward, add_rms_norm_quant_forward, counter_dropout_forward, drop_threshold,
                        dropout_rng, fused_dynamic_weights_forward, hc_mix_forward, hc_mix_norm_forward,
-                       meanpool_forward, sinkhorn_forward, stream_mix_forward, stream_norm_forward,
+                       meanpool_forward, row_number, sinkhorn_forward, stream_mix_forward, stream_norm_forward,
                        stream_norm_quant_forward)
 
 
@@ -410,7 +410,7 @@ def add_residual_from_state(stand_in, H, H_res, branch_output, H_post, pool_for_
 def _add_residual_dropout(carrier, H, H_res, branch_output, H_post, pool_for_next, rng, threshold, row_offset):
     rng = dropout_rng(rng, branch_output)
     out = _AddResidualDropout.apply(carrier, H, H_res, branch_output, H_post, bool(pool_for_next), rng, threshold,
-                                    int(row_offset))
+                                    row_number(row_offset))
     if not pool_for_next:
         return out
     H_new, partials = out
@@ -503,8 +503,8 @@ def counter_dropout(x: torch.Tensor, p: float, rng=None, row_offset: int = 0) ->
         return x
     rng = dropout_rng(rng, x)
     if not _records(x):
-        return counter_dropout_forward(x, rng, threshold, int(row_offset))
-    return _CounterDropout.apply(x, rng, threshold, int(row_offset))
+        return counter_dropout_forward(x, rng, threshold, row_number(row_offset))
+    return _CounterDropout.apply(x, rng, threshold, row_number(row_offset))
 
 
 @torch.compiler.disable
@@ -519,9 +519,9 @@ def fused_add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None,
     threshold = drop_threshold(dropout_p)
     rng = dropout_rng(rng, x) if threshold else None
     if not _records(x, residual, weight):
-        y, s, _ = add_rms_norm_forward(x, residual, weight, eps, rng, threshold, int(row_offset), want_rstd=False)
+        y, s, _ = add_rms_norm_forward(x, residual, weight, eps, rng, threshold, row_number(row_offset), want_rstd=False)
         return y, (s if residual is not None or threshold else x)
-    out = _AddRmsNorm.apply(x, residual, weight, eps, rng, threshold, int(row_offset))
+    out = _AddRmsNorm.apply(x, residual, weight, eps, rng, threshold, row_number(row_offset))
     return out if isinstance(out, tuple) else (out, x)
 
 
