@@ -263,16 +263,20 @@ int mhc_rms_norm_bwd(const void* dy, const void* dsum, const void* x, const void
                      int64_t scratch_bytes, int64_t rows, int64_t D, int dtype, mhc_stream_t stream);
 
 /* Norm of the mixed streams in the kernel that mixes them: b = sum_n H_pre[n] H[n]; y = norm(b) * weight.
- * branch_input (b rounded to the activation type; where it is written, the rounded b is what is normalised) and
- * rstd [B, S] may be NULL.  Fuses the first half of
- * stream_mix_forward (src/mhc/_kernels.py:617-652) with the norm its caller runs on branch_input. */
+ * branch_input (b rounded to the activation type) and rstd [B, S] may be NULL.  Where branch_input is written, the
+ * rounded b is what is normalised and what rstd belongs to; that forward's backward is mhc_rms_norm_bwd on
+ * branch_input, followed by a backward of the mix (mhc_hc_mix_bwd, or mhc_stream_mix_bwd with a gradient of zero for the
+ * residual mix).  mhc_stream_norm_bwd forms the unrounded b again and belongs to a forward with branch_input == NULL.
+ * Fuses the first half of stream_mix_forward (src/mhc/_kernels.py:617-652) with the norm its caller runs on
+ * branch_input. */
 int mhc_stream_norm_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype,
                         void* branch_input, void* y, float* rstd, int64_t B, int64_t S, int64_t D, int dtype,
                         float eps, mhc_stream_t stream);
 int mhc_stream_norm_quant_fwd(const void* H, const float* H_pre, const void* weight, int weight_dtype, void* q,
                               void* scales, int64_t group, int scale_type, int64_t B, int64_t S, int64_t D,
                               int dtype, float eps, mhc_stream_t stream);
-/* dH [B,S,4,D], dH_pre [B,4] fp32 and dweight (may be NULL) from dy and H; the mix is recomputed. */
+/* dH [B,S,4,D], dH_pre [B,4] fp32 and dweight (may be NULL) from dy, H and the rstd of a forward without
+ * branch_input; the mix is recomputed. */
 int mhc_stream_norm_bwd(const void* dy, const void* H, const float* H_pre, const float* rstd,
                         const void* weight, int weight_dtype, void* dH, float* dH_pre, void* dweight,
                         void* scratch, int64_t scratch_bytes, int64_t B, int64_t S, int64_t D, int dtype,

@@ -237,7 +237,7 @@ def rms_norm_backward(dy, dsum, x, residual, rstd, weight=None, rng=None, thresh
 
 
 def stream_norm_backward(dy, H, H_pre, rstd, weight=None, want_dweight: bool = True):
-    """(dH, dH_pre [B,4] fp32, dweight or None) of stream_norm_forward."""
+    """(dH, dH_pre [B,4] fp32, dweight or None) of stream_norm_forward without want_branch_input."""
     B, S, n, D = H.shape
     _check(n == 4 and dy.shape == (B, S, D) and H_pre.shape == (B, 4) and rstd.numel() == B * S, "shape mismatch")
     dev = L.same_device(H, dy, H_pre, rstd, weight)

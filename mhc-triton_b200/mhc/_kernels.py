@@ -355,7 +355,9 @@ def _stream_inputs(H, H_pre, weight):
 
 def stream_norm_forward(H, H_pre, weight=None, eps: float = 1e-6, want_branch_input: bool = False,
                         want_rstd: bool = True):
-    """(y, branch_input or None, rstd [B*S]): branch_input = sum_n H_pre[n] H[n], y its norm times weight."""
+    """(y, branch_input or None, rstd [B*S]): branch_input = sum_n H_pre[n] H[n], y its norm times weight.  With
+    want_branch_input y is the norm of the stored (rounded) branch_input: its backward is rms_norm_backward on that and then
+    the mix's; stream_norm_backward belongs to the form without."""
     dev, H, H_pre, (w, wcode, wptr) = _stream_inputs(H, H_pre, weight)
     B, S, _, D = H.shape
     y = torch.empty((B, S, D), device=H.device, dtype=H.dtype)
