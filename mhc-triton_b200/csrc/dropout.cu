@@ -9,7 +9,8 @@ namespace mhc {
 // A thread owns one 16-byte pack of columns and walks kDropRows rows: the column's part of the generator is computed once
 // and all loads are issued before the first use.  Bound by the generator's instructions (ALU pipe 58 %, 2.9 of 4 issue
 // slots): 92 us at 32768 x 4096 bf16, 5.8 TB/s.  4 or 6 rows take 96, 5 or 7 CTAs per SM 102 or 99, a shared-memory ring
-// over 8 to 32 rows 105 to 120.
+// over 8 to 32 rows 105 to 120.  fp32, where two threads compute the same block for four columns each: 48 us at 8192 x 4096
+// (41 at the memory's rate), 90 at 8192 x 8192 (82).
 #ifndef MHC_DROPOUT_MINB
 #define MHC_DROPOUT_MINB 6
 #endif

@@ -7,7 +7,9 @@
 // dweight = sum_rows dy s rstd; dropout's mask is recomputed.  All sums, the norm and the scales are fp32.  s is
 // normalised as computed, before it is rounded to the activation type for sum_out, and the backward forms it again
 // from x and residual instead of reading the rounded sum_out: one more tensor to read (5 instead of 4 of a bf16
-// backward's moves), but dweight keeps fp32 accuracy (from the rounded sums it is off by 1e-3).  Where the mix is
+// backward's moves), but dweight keeps fp32 accuracy (from the rounded sums it is off by 1e-3).  It is a sum in fp32 over the
+// rows a CTA walks and in fp64 above that: off by 1.3e-7 of the columns' root mean square in the median and 8e-7 at most at
+// 32768 x 4096 bf16 (fp64 throughout: 4e-8 and 2.6e-7; the row's own roundings).  Where the mix is
 // stored as branch_input, the stored value is what is normalised, so its backward, which reads it, is exact too.
 #include <algorithm>
 #include <atomic>
@@ -173,7 +175,9 @@ __device__ __forceinline__ void block_sum_max(float& sum, float& mx, float* sm) 
   mx = m;
 }
 
-// -------------------------------------------------------- rows too wide for registers (over 16384, or 8192 odd or unaligned)
+// ------------------------------------------ rows too wide for registers (16-bit types over 16384 columns; fp32, odd or
+// unaligned ones over 8192).  Read element by element, twice, and dweight is updated in memory: right, not fast.  4096 x 32768
+// bf16 with a residual 484 us forward (164 at the memory's rate) and 2548 backward (205); fp32 4096 x 16384 270 and 925.
 // s[row, d], read element by element.
 template <typename T, Src SRC, bool DROP>
 __device__ __forceinline__ float src_at(const NormFwd& a, const DropSeed& seed, const float (&pre)[4], int64_t row, int64_t d) {
@@ -722,6 +726,10 @@ k_norm_fwd_ring(NormFwd a, RowMap m) {
 // elements, which cp.async cannot copy): loads straight from memory.  204 us at 32768 x 4096 bf16 (five tensors, 6.6 TB/s),
 // 118 at 8192 x 7168 with dropout (six, 6.0 TB/s, bound by instructions: 14 warps per SM and twice as many per pack), 108
 // for the streams at 2 x 4096 x 4096 (nine, 5.6 TB/s).  One pack per thread and twice the warps was no faster.
+// Two instances have more values than registers and spill: four packs of 16-bit values per thread (rows of 8193 to 16384 columns;
+// 216 bytes of stores, 472 for the streams, 660 with dropout; 273 us at 8192 x 16384 bf16, 205 at the memory's rate, 443
+// with dropout, 258 for the streams at 2 x 2048 x 16384, 185) and single elements in more than 512 threads (4097 to 8192 columns;
+// 248, 456 for the streams; 272 us at 8192 x 6001 bf16, 75 at the memory's rate).
 template <typename T, int V, int NP, int DEPTH, int THREADS, Src SRC, bool DROP>
 __global__ void __launch_bounds__(THREADS)
 k_norm_bwd(NormBwd a, RowMap m) {

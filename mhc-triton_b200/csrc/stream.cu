@@ -183,7 +183,8 @@ k_stream_premix_fwd(const T* __restrict__ H, const float* __restrict__ Hpre, T* 
 // The forms with dropout take 3 times as many instructions per pack; loads in registers then leave too few warps to cover
 // both the memory and the generator's chain of multiplications (397 / 329 us forward / backward at 8 x 4096 x 4096
 // bf16, 357 / 247 without dropout).  They keep MHC_DROP_STAGES tokens in the shared-memory ring instead and walk more
-// tokens per CTA: 349 / 263 us.
+// tokens per CTA: 349 / 263 us.  The form that recomputes H_res @ H (k_add_residual_mix_fwd) needs no ring: one token per
+// thread and many short CTAs cover the generator as they are.
 #ifndef MHC_DROP_STAGES
 #define MHC_DROP_STAGES 3
 #endif
@@ -361,7 +362,9 @@ k_add_residual_pool_fwd(const T* __restrict__ Hr, const T* __restrict__ bo, cons
 // recomputed from H here instead of being written by the stream-mix kernel and read back (saves
 // 8 of the 46 D*e bytes per token of a layer step).  The sum is formed first and the branch term
 // added last, the order the two separate kernels use.  POOL: also leave the per-chunk token sums
-// of H_new for the next layer (see k_add_residual_pool_fwd).
+// of H_new for the next layer (see k_add_residual_pool_fwd).  Bound by memory, with dropout as well: 353 us without and
+// 363 with it at 8 x 4096 x 4096 bf16 (nine tensors, 369 at the rate of a copy), 169 and 162 at 2 x 4096 x 7168 (161); pooling
+// 389 and 395, 182 and 185.
 #ifndef MHC_TPC_ADDMIX
 #define MHC_TPC_ADDMIX 1
 #endif
