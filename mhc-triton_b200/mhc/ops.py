@@ -178,23 +178,24 @@ def _first_order(depends, applies=lambda ctx: True):
     are differentiated or the gradients depend on the node's own differentiated inputs (`depends(ctx, *grads)`).  Elsewhere
     they are constants; an upstream gradient that is handed through stays what it is.  Nodes for which `applies` is false run
     `backward` as it is."""
-    return lambda backward: functools.partial(_run_first_order, backward, depends, applies)
-
-
-def _run_first_order(backward, depends, applies, ctx, *grads):
-    if not (torch.is_grad_enabled() and applies(ctx)):
-        return backward(ctx, *grads)
-    with torch.no_grad():
-        out = backward(ctx, *grads)
-    given = [g for g in grads if g is not None]
-    if not depends(ctx, *grads) and not any(g.requires_grad for g in given):
-        return out
-    which = [i for i, o in enumerate(out) if o is not None and not any(o is g for g in given)]
-    if not which:
-        return out
-    anchor = torch.empty(0, device=out[which[0]].device, requires_grad=True)
-    marked = dict(zip(which, _NoSecondDerivative.apply(anchor, *[out[i] for i in which])))
-    return tuple(marked.get(i, o) for i, o in enumerate(out))
+    def decorate(backward):
+        @functools.wraps(backward)
+        def run(ctx, *grads):
+            if not (torch.is_grad_enabled() and applies(ctx)):
+                return backward(ctx, *grads)
+            with torch.no_grad():
+                out = backward(ctx, *grads)
+            given = [g for g in grads if g is not None]
+            if not depends(ctx, *grads) and not any(g.requires_grad for g in given):
+                return out
+            which = [i for i, o in enumerate(out) if o is not None and not any(o is g for g in given)]
+            if not which:
+                return out
+            anchor = torch.empty(0, device=out[which[0]].device, requires_grad=True)
+            marked = dict(zip(which, _NoSecondDerivative.apply(anchor, *[out[i] for i in which])))
+            return tuple(marked.get(i, o) for i, o in enumerate(out))
+        return run
+    return decorate
 
 
 class _HyperConnectionMix(torch.autograd.Function):
